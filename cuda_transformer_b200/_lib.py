@@ -61,6 +61,9 @@ class DecayRuns(C.Structure):
 ZERO1_SYNC_BYTES = 1024
 SYNC_SIGNAL, SYNC_WAIT, SYNC_ADVANCE, SYNC_STAMP = 1, 2, 4, 8
 PHASE_GRADS, PHASE_PAIRS, PHASE_WEIGHTS = 0, 1, 2
+F16, BF16, F32 = 0, 1, 2
+LOSS_WORKSPACE_BYTES = 32768
+MAX_LISTED, MAX_EXPERTS = 1024, 1024
 
 assert C.sizeof(StepState) == 60 and C.sizeof(ScheduleConfig) == 44 and C.sizeof(TensorInfo) == 24
 assert C.sizeof(Zero1Sync) == 72
@@ -69,6 +72,7 @@ _P = C.c_void_p
 _LL = C.c_longlong
 _I = C.c_int
 _F = C.c_float
+_D = C.c_double
 
 # name -> (restype, argtypes); every symbol include/b200amp.h declares
 PROTOTYPES = {
@@ -109,6 +113,11 @@ PROTOTYPES = {
     "b200amp_pass2_ag_f16_ce": (_I, [_P, _P, _P, _P, _P, _I, _I, _LL, _LL, _P, _I, _P, _F, _F, _F, _I, _P]),
     "b200amp_step_f16": (_I, [_P, _P, _P, _P, _P, _LL, _P, _I, _P, _P, C.POINTER(ScheduleConfig), _P, _I,
                               _F, _F, _F, _P]),
+    "b200amp_loss_workspace_init": (_I, [_P, _P]),
+    "b200amp_top_logits": (_I, [_P, _I, _LL, _I, _LL, _I, _D, _P, _P, _P, _P]),
+    "b200amp_distill_loss": (_I, [_P, _LL, _P, _LL, _I, _LL, _I, _I, _P, _P, _I, _P, _P, _I, _D, _D, _D, _P, _P, _P,
+                                  _P]),
+    "b200amp_balance_loss": (_I, [_P, _LL, _P, _LL, _I, _LL, _I, _P, _I, _P, _D, _I, _I, _P, _P, _P, _P, _P]),
     "b200amp_graph_begin_capture": (_I, [_P]),
     "b200amp_graph_end_capture": (_I, [_P, C.POINTER(_P)]),
     "b200amp_graph_launch": (_I, [_P, _P]),

@@ -32,6 +32,7 @@ import torch
 from . import _lib
 from ._lib import B200AmpError, DecayRuns, ScheduleConfig, StepState, TensorInfo, Zero1Sync, check
 from .layout import ParamSlot, padded, shard_range, tensor_table
+from .losses import LossCalls, loss_workspace
 
 __all__ = [
     "StepState", "ScheduleConfig", "TensorInfo", "B200AmpError",
@@ -471,7 +472,7 @@ class HostGradientFeed:
         f["step"].synchronize()
 
 
-class AmpOptimizer(HostGradientFeed):
+class AmpOptimizer(HostGradientFeed, LossCalls):
     """The optimizer state of one GPU that holds the whole arena.
 
     Arenas (flat, in param_layout order, cuda/gpt_fast.cu:96-115): master, m, v (fp32),
@@ -505,6 +506,7 @@ class AmpOptimizer(HostGradientFeed):
             self.state = torch.zeros(C.sizeof(StepState), dtype=torch.uint8, device=self.device)
             self.history = torch.zeros(C.sizeof(StepState) * history_len, dtype=torch.uint8, device=self.device)
             self.workspace = torch.zeros(self.lib.b200amp_workspace_bytes(), dtype=torch.uint8, device=self.device)
+            self.loss_workspace = loss_workspace(self.device)
         self.reset(loss_scale)
 
     @staticmethod
@@ -719,8 +721,9 @@ def initial_state_host(scale: float) -> StepState:
     return st
 
 
-class ShardedAmpOptimizer(Zero1Step):
-    """Zero1Step bound to the CUDA kernels: one rank per B200, NCCL process group."""
+class ShardedAmpOptimizer(Zero1Step, LossCalls):
+    """Zero1Step bound to the CUDA kernels: one rank per B200, NCCL process group. The losses write this
+    rank's mean into this rank's state, and their gradients average over the ranks as any others do."""
 
     def __init__(self, slots: List[ParamSlot], cfg: ScheduleConfig, eps: float = 1e-8,
                  loss_scale: float = 65536.0, history_len: int = 256, device=None, group=None):
@@ -733,6 +736,7 @@ class ShardedAmpOptimizer(Zero1Step):
             super().__init__(slots, cfg, eps, loss_scale, history_len, device, group)
             self.tensors = _tensor_table_device(self.table, self.device, self.n)
             self.workspace = torch.zeros(self.lib.b200amp_workspace_bytes(), dtype=torch.uint8, device=self.device)
+            self.loss_workspace = loss_workspace(self.device)
             # pass 1 publishes {sum, flag} in the first 16 bytes of its workspace
             self.sums_local = self.workspace[:16].view(torch.float64)
 

@@ -83,8 +83,8 @@ typedef struct b200amp_step_state
     float step_size;        /* lr / (1 - beta1^t) */
     float bc2_sqrt;         /* sqrt(1 - beta2^t) */
     float decay;            /* 1 - lr * weight_decay */
-    float loss;             /* written by the caller's forward pass; carried, never read here */
-    int n_valid;            /* written by the caller's forward pass; carried, never read here */
+    float loss;             /* written by the forward pass (the caller's, or the losses below); carried by the step */
+    int n_valid;            /* written by the forward pass (the caller's, or the losses below); carried by the step */
 } b200amp_step_state;
 
 typedef struct b200amp_schedule
@@ -405,6 +405,92 @@ B200AMP_API int b200amp_step_f16(float *master, float *m, float *v, const void *
                      const b200amp_tensor_info *tensors, int ntensors, b200amp_step_state *st, void *workspace,
                      const b200amp_schedule *cfg, b200amp_step_state *history, int history_len,
                      float beta1, float beta2, float eps, b200amp_stream s);
+
+/* ---------------------------------------------------------------- losses that open the backward pass
+ * What stands before the step: the forward pass ends in a loss, and the loss's gradient, multiplied by
+ * st->loss_scale, is what the backward pass starts from. The step state has two fields for it (loss,
+ * n_valid: the finalize carries them into the history ring); these operators write them. The reference
+ * has the plain cross-entropy of one label a row (cuda/kernels/crossentropy.cu, cuda/kernels/fused.cu:336-449);
+ * its other losses have no counterpart there.
+ *
+ * Matrices are rows of `cols` elements, `ld` elements from one row to the next; any alignment of the
+ * element type is taken, and rows that start on 16-byte boundaries are fastest. dtype is one of the
+ * three below. Nothing is allocated; every array is device memory of the current device. Sums and
+ * statistics are held in fp32 or fp64; a gradient is rounded once, to its own type. The results depend
+ * on the inputs and the shapes alone, never on the order in which blocks finish, so a replay gives the
+ * same bits. A gradient beyond the type's range becomes inf and skips the step, as any other would.
+ *
+ * The workspace is B200AMP_LOSS_WORKSPACE_BYTES bytes, 16-byte aligned, zeroed once (cudaMemset or
+ * b200amp_loss_workspace_init); the kernels leave its counters at zero again. One workspace serves one
+ * stream at a time: calls whose GPU work may overlap (two streams, two graphs replayed side by side) need one each. */
+enum
+{
+    B200AMP_F16 = 0,
+    B200AMP_BF16 = 1,
+    B200AMP_F32 = 2
+};
+#define B200AMP_LOSS_WORKSPACE_BYTES 32768
+#define B200AMP_MAX_LISTED 1024     /* most listed logits a row (k of the two entry points below) */
+#define B200AMP_MAX_EXPERTS 1024    /* most experts of a router */
+B200AMP_API int b200amp_loss_workspace_init(void *workspace, b200amp_stream s);
+
+/* A teacher's record: of every row the k largest of the first `vocab` columns in descending order, ties
+ * to the lowest column, with their columns, and (lse not null) log sum_v exp(z_v / temperature) over all
+ * of them. values[rows][k] has the type of the logits (the values are copied, not rounded),
+ * indices[rows][k] is int32, lse[rows] fp32. NaN counts as larger than any number and -0 equals +0.
+ * k > vocab: the entries behind the last column get index -1 and value -inf, which b200amp_distill_loss
+ * leaves out. rows >= 0, 1 <= k <= 1024, 1 <= vocab <= ld. No reference counterpart. */
+B200AMP_API int b200amp_top_logits(const void *logits, int dtype, long long rows, int vocab, long long ld, int k,
+                                   double temperature, void *values, int *indices, float *lse, b200amp_stream s);
+
+/* Distillation from a teacher's top logits, mixed with the cross-entropy of a label, forward and backward.
+ * Row i has student logits z (columns 0 .. vocab - 1; columns vocab .. cols - 1 pad the vocabulary: they
+ * are not read and get gradient 0), a label y = targets[i], and k listed teacher logits t_j at columns
+ * indices[i][j]. With q = softmax(z / T), T = temperature:
+ *     lse given:  p_j = exp(t_j / T - lse_i)   and rest = max(0, 1 - sum_j p_j) for all columns not listed
+ *     lse null:   p   = softmax over the listed t_j / T, rest = 0
+ *     KL_i  = sum_j p_j log(p_j / q_j) + rest log(rest / sum of q over the columns not listed)
+ *     loss_i = soft_weight * KL_i - hard_weight * log softmax(z)_y
+ * (the usual T^2 is the caller's, in soft_weight). loss_i goes to row_loss[i] (fp32), the gradient of
+ * (1 / n_valid) sum_i loss_i times st->loss_scale to dlogits, the mean to st->loss and the number of rows
+ * that count to st->n_valid; n_valid == 0 gives loss 0.
+ *   - targets[i] < 0: the row does not count: loss 0, gradient 0. targets may be null when hard_weight is
+ *     0: every row counts. With hard_weight 0 the label says only whether the row counts.
+ *   - indices < 0 are empty slots. A row without any listed mass has KL 0. A column listed twice has the
+ *     sum of its masses. If the student gives every column not listed no probability at all (or there
+ *     is none), the rest term is left out.
+ *   - An index or a label beyond the vocabulary is not read: the row's loss and gradient are NaN, so the
+ *     step is skipped. NaN, +inf or nothing but -inf in a row of logits, or NaN in its record, do the
+ *     same. A single -inf logit has probability 0 and gradient 0; where it has teacher mass or is the
+ *     label, the loss is +inf and the gradient finite.
+ *   - k == 0 or soft_weight == 0: the cross-entropy alone (values, indices and lse may be null).
+ *   - dlogits null: the loss alone. dlogits may be the logits themselves (same ld).
+ * values[rows][k] has type value_dtype, indices[rows][k] int32, lse[rows] fp32. rows >= 0, 0 <= k <= 1024,
+ * 1 <= vocab <= cols <= ld and dld, T > 0, finite weights. Reference: the label's part is
+ * cuda/kernels/crossentropy.cu:16-82; the teacher's has no counterpart. */
+B200AMP_API int b200amp_distill_loss(const void *logits, long long ld, void *dlogits, long long dld, int dtype,
+                                     long long rows, int vocab, int cols, const int *targets, const void *values,
+                                     int value_dtype, const int *indices, const float *lse, int k, double temperature,
+                                     double soft_weight, double hard_weight, b200amp_step_state *st, float *row_loss,
+                                     void *workspace, b200amp_stream s);
+
+/* The balance loss of a mixture-of-experts router, with the per-expert counts and the gradient. Row i has
+ * router logits z (one column an expert) and k chosen experts chosen[i][0..k-1] (negative: a choice not
+ * made). Over the n rows that count (targets null, or targets[i] >= 0):
+ *     counts[e] = choices of expert e,  f_e = counts[e] / (n k),  p_i = softmax(z_i)
+ *     loss = weight * experts * sum_e f_e (1/n) sum_i p_ie
+ * The counts are constants of the gradient. loss[0] = loss (fp32); dlogits = gradient * st->loss_scale
+ * (rows that do not count: 0), or, with accumulate != 0, is added to what dlogits holds (rows that do not
+ * count: left as they are). add_to_state != 0 also adds the loss to st->loss (st->n_valid is not
+ * touched), for a loss that joins the model's: call it after the one that writes st->loss. n == 0: loss 0.
+ * An expert beyond the last is not counted and makes the loss and every gradient NaN. dlogits may be null
+ * (the counts and the loss alone) or the logits themselves (accumulate == 0, same ld).
+ * rows >= 0, 1 <= experts <= 1024, experts <= ld and dld, 1 <= k <= 1024, rows * k < 2^31. At most two
+ * launches. No reference counterpart (its models have no experts). */
+B200AMP_API int b200amp_balance_loss(const void *logits, long long ld, void *dlogits, long long dld, int dtype,
+                                     long long rows, int experts, const int *chosen, int k, const int *targets,
+                                     double weight, int accumulate, int add_to_state, b200amp_step_state *st,
+                                     int *counts, float *loss, void *workspace, b200amp_stream s);
 
 /* ---------------------------------------------------------------- CUDA-graph helpers
  * Replace CudaGraph::{capture,launch} and its destructor (cuda/graph.h:14-30,

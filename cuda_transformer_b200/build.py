@@ -25,6 +25,7 @@ SOURCES = ["api.cu", "scaler.cu", "adamw.cu", "pass2.cu", "zero1.cu",
            "distill.cu", "top_logits.cu", "balance.cu"]
 HEADERS = [os.path.join(CSRC_DIR, "internal.cuh"), os.path.join(CSRC_DIR, "adamw_math.cuh"),
            os.path.join(CSRC_DIR, "pass1_common.cuh"), os.path.join(CSRC_DIR, "loss_common.cuh"),
+           os.path.join(CSRC_DIR, "row_tile.cuh"),
            os.path.join(INCLUDE_DIR, "b200amp.h")]
 
 NVCC_FLAGS = [

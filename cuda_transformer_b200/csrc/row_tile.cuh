@@ -1,0 +1,335 @@
+// row_tile.cuh: one row of a matrix held in the shared memory of a thread-block cluster.
+//
+// A vocabulary row is swept several times (maximum, sums, gradient) but should cross HBM once each way. The C
+// blocks of a cluster take a segment of the row each (C = 1: the whole row) and keep it in shared memory between
+// the sweeps; what the segments have to tell each other goes through distributed shared memory. A segment sits at the
+// same offset from a 16-byte boundary as in global memory, so that all but its two ends moves in 16-byte accesses
+// whatever the row's alignment.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include <mutex>
+
+#include "loss_common.cuh"
+
+namespace b200amp
+{
+
+constexpr int MAX_CLUSTER = 16;
+constexpr int MAX_ROW_SMEM = 220 * 1024;        // dynamic shared memory of a block at most
+
+// How a matrix is spread: decided on the host, the same for every row.
+struct RowPlan
+{
+    int cluster;            // blocks a row
+    int segment;            // columns a block, a multiple of 64
+    int threads;
+    int smem;               // dynamic shared memory of a block
+};
+
+// Cluster and block size for rows of `cols` elements of `size` bytes, with `more` bytes of shared memory
+// besides the segment. B200AMP_ERR_LIMIT where a row does not fit the largest cluster.
+inline int plan_rows(long long rows, int cols, int size, int more, RowPlan *plan)
+{
+    const int sms = sm_count();
+    if (sms <= 0)
+    {
+        return B200AMP_ERR_CUDA;
+    }
+    auto fill = [&](int cluster) {
+        plan->cluster = cluster;
+        plan->segment = static_cast<int>(((static_cast<long long>(cols) + cluster - 1) / cluster + 63) / 64 * 64);
+        plan->smem = ((plan->segment * size + 31) & ~15) + ((more + 15) & ~15) + plan->segment / 8;
+    };
+    plan->threads = 256;
+    int cluster = 1;
+    if (static_cast<long long>(cols) * size > MAX_CLUSTER * static_cast<long long>(MAX_ROW_SMEM))
+    {
+        set_error("rows of %d columns are beyond the maximum of %lld", cols, MAX_CLUSTER * static_cast<long long>(MAX_ROW_SMEM) / size);
+        return B200AMP_ERR_LIMIT;
+    }
+    for (fill(1); cluster < MAX_CLUSTER && plan->smem > 55 * 1024; fill(cluster))
+    {
+        cluster *= 2;
+    }
+    while (cluster < MAX_CLUSTER && rows * cluster < sms && plan->segment > 2048)
+    {
+        cluster *= 2;
+        fill(cluster);
+    }
+    if (plan->segment * size <= 12 * 1024)
+    {
+        plan->threads = 128;
+    }
+    if (plan->smem > MAX_ROW_SMEM)
+    {
+        set_error("rows of %d columns need %d bytes of shared memory a block", cols, plan->smem);
+        return B200AMP_ERR_LIMIT;
+    }
+    return B200AMP_OK;
+}
+
+#ifdef __CUDACC__
+
+template <typename T>
+struct Vec16                // 16 bytes of a row
+{
+    static constexpr int N = 16 / sizeof(T);
+    uint4 w;
+};
+
+// the elements as pairs of floats
+__device__ __forceinline__ void unpack(const Vec16<__half> &v, float2 (&f)[4])
+{
+    const uint32_t words[4] = {v.w.x, v.w.y, v.w.z, v.w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        f[i] = half2_bits_to_float2(words[i]);
+    }
+}
+__device__ __forceinline__ void unpack(const Vec16<__nv_bfloat16> &v, float2 (&f)[4])
+{
+    const uint32_t words[4] = {v.w.x, v.w.y, v.w.z, v.w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        f[i] = make_float2(__uint_as_float(words[i] << 16), __uint_as_float(words[i] & 0xFFFF0000u));
+    }
+}
+__device__ __forceinline__ void unpack(const Vec16<float> &v, float2 (&f)[2])
+{
+    f[0] = make_float2(__uint_as_float(v.w.x), __uint_as_float(v.w.y));
+    f[1] = make_float2(__uint_as_float(v.w.z), __uint_as_float(v.w.w));
+}
+
+__device__ __forceinline__ void pack(Vec16<__half> &v, const float2 (&f)[4])
+{
+    v.w = make_uint4(float2_to_half2_bits(f[0].x, f[0].y), float2_to_half2_bits(f[1].x, f[1].y),
+                     float2_to_half2_bits(f[2].x, f[2].y), float2_to_half2_bits(f[3].x, f[3].y));
+}
+__device__ __forceinline__ uint32_t bf16_pair(float2 f)
+{
+    __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<uint32_t *>(&b);
+}
+__device__ __forceinline__ void pack(Vec16<__nv_bfloat16> &v, const float2 (&f)[4])
+{
+    v.w = make_uint4(bf16_pair(f[0]), bf16_pair(f[1]), bf16_pair(f[2]), bf16_pair(f[3]));
+}
+__device__ __forceinline__ void pack(Vec16<float> &v, const float2 (&f)[2])
+{
+    v.w = make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+}
+
+// maximum with NaN winning, pair by pair in the element type
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __half)
+{
+    __half2 r = __hmax2_nan(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    return *reinterpret_cast<uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, __nv_bfloat16)
+{
+    __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+    return *reinterpret_cast<uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b, float)
+{
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+}
+template <typename T>
+__device__ __forceinline__ void max_into(Vec16<T> &m, const Vec16<T> &v)
+{
+    m.w.x = max2_nan(m.w.x, v.w.x, T());
+    m.w.y = max2_nan(m.w.y, v.w.y, T());
+    m.w.z = max2_nan(m.w.z, v.w.z, T());
+    m.w.w = max2_nan(m.w.w, v.w.w, T());
+}
+template <typename T>
+__device__ __forceinline__ float max_of(const Vec16<T> &v)
+{
+    float2 f[Vec16<T>::N / 2];
+    unpack(v, f);
+    float m = max_nan(f[0].x, f[0].y);
+#pragma unroll
+    for (int i = 1; i < Vec16<T>::N / 2; i++)
+    {
+        m = max_nan(m, max_nan(f[i].x, f[i].y));
+    }
+    return m;
+}
+
+template <typename T>
+__device__ __forceinline__ T minus_infinity()
+{
+    return from_float<T>(-INFINITY);
+}
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(r))
+        : "l"(reinterpret_cast<unsigned long long &>(a)), "l"(reinterpret_cast<unsigned long long &>(b)),
+          "l"(reinterpret_cast<unsigned long long &>(c)));
+    return r;
+}
+
+__device__ __forceinline__ void copy_async16(void *dst_smem, const void *src_gmem)
+{
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;"
+                 :
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst_smem))), "l"(src_gmem)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_async_wait()
+{
+    asm volatile("cp.async.wait_all;" : : : "memory");
+}
+
+// This block's segment of the current row.
+template <typename T, int THREADS>
+struct RowTile
+{
+    static constexpr int N = Vec16<T>::N;
+    char *buf;              // 16-byte aligned: segment * sizeof(T) + 16 bytes
+    int first;              // first column of the segment
+    int lead;               // elements between buf and the first column's place (0 .. N - 1)
+    int valid, held;        // columns of the segment that hold logits, and with the padding behind them
+    int vecs;               // 16-byte vectors to sweep; what is in none of the columns holds -inf
+
+    __device__ __forceinline__ T *at(int column)            // of this segment, in shared memory
+    {
+        return reinterpret_cast<T *>(buf) + lead + (column - first);
+    }
+    __device__ __forceinline__ bool holds(int column) const
+    {
+        return column >= first && column < first + valid;
+    }
+    __device__ __forceinline__ Vec16<T> vec(int i) const
+    {
+        return reinterpret_cast<const Vec16<T> *>(buf)[i];
+    }
+
+    // Starts the copy of columns [first, first + valid) of the row at z; padding and ends are set to -inf.
+    // Every thread; the row is there after copy_async_wait and a barrier.
+    __device__ __forceinline__ void start(const T *z, int first_column, int segment, int vocab, int cols)
+    {
+        first = first_column;
+        valid = max(0, min(segment, vocab - first));
+        held = max(0, min(segment, cols - first));
+        const char *src = reinterpret_cast<const char *>(z + first);
+        const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(src) & 15);
+        lead = skew / static_cast<int>(sizeof(T));
+        vecs = held > 0 ? (lead + held + N - 1) / N : 0;
+        const int whole_first = lead > 0 ? 1 : 0, whole_end = (lead + valid) / N;      // vectors inside the columns
+        src -= skew;
+        for (int i = whole_first + threadIdx.x; i < whole_end; i += THREADS)
+        {
+            copy_async16(buf + 16 * i, src + 16ll * i);
+        }
+        // the elements of the other vectors: at most N - 1 at the front, then the end and the padding
+        T *e = reinterpret_cast<T *>(buf);
+        const T *g = reinterpret_cast<const T *>(src);
+        const int front = whole_first * N, back = max(front, whole_end * N);
+        for (int i = threadIdx.x; i < front + (vecs * N - back); i += THREADS)
+        {
+            const int k = i < front ? i : back + i - front;
+            e[k] = k >= lead && k < lead + valid ? g[k] : minus_infinity<T>();
+        }
+    }
+};
+
+// Blocks of a kernel that fit the device at once, as whole clusters (asked once for each shape).
+template <typename Kernel>
+int resident_clusters(Kernel kernel, const RowPlan &plan, int *clusters)
+{
+    struct Known
+    {
+        const void *kernel;
+        int device, cluster, smem, clusters;
+    };
+    static std::mutex lock;
+    static Known known[64];
+    static int count = 0;
+    int device = 0;
+    B200AMP_CUDA(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> hold(lock);
+    for (int i = 0; i < count && i < 64; i++)
+    {
+        if (known[i].kernel == reinterpret_cast<const void *>(kernel) && known[i].device == device && known[i].cluster == plan.cluster && known[i].smem == plan.smem)
+        {
+            *clusters = known[i].clusters;
+            return B200AMP_OK;
+        }
+    }
+    B200AMP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_ROW_SMEM));
+    B200AMP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(plan.cluster);
+    config.blockDim = dim3(plan.threads);
+    config.dynamicSmemBytes = plan.smem;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim = {static_cast<unsigned>(plan.cluster), 1u, 1u};
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    int n = 0;
+    B200AMP_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &config));
+    if (n < 1)
+    {
+        set_error("no cluster of %d blocks with %d bytes of shared memory fits the device", plan.cluster, plan.smem);
+        return B200AMP_ERR_CUDA;
+    }
+    known[count % 64] = {reinterpret_cast<const void *>(kernel), device, plan.cluster, plan.smem, n};
+    count++;
+    *clusters = n;
+    return B200AMP_OK;
+}
+
+template <typename Kernel, typename Args>
+int launch_rows(Kernel kernel, const Args &args, RowPlan plan, long long rows, cudaStream_t stream)
+{
+    int clusters = 0;
+    const int rc = resident_clusters(kernel, plan, &clusters);
+    if (rc != B200AMP_OK)
+    {
+        return rc;
+    }
+    clusters = static_cast<int>(rows < 1 ? 1 : rows < clusters ? rows : clusters);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(clusters * plan.cluster);
+    config.blockDim = dim3(plan.threads);
+    config.dynamicSmemBytes = plan.smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim = {static_cast<unsigned>(plan.cluster), 1u, 1u};
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    B200AMP_CUDA(cudaLaunchKernelEx(&config, kernel, args, plan));
+    B200AMP_LAUNCHED();
+    return B200AMP_OK;
+}
+
+#endif // __CUDACC__
+
+} // namespace b200amp

@@ -34,6 +34,17 @@ struct DistillArgs
     LossWorkspace *ws;
 };
 
+// Places of the table that finds columns listed twice: a power of two, at least twice the listed ones.
+__host__ __device__ inline int distill_table(int k)
+{
+    int n = 2;
+    while (n < 2 * k)
+    {
+        n *= 2;
+    }
+    return n;
+}
+
 // Rows that count: every block counts for itself, as the gradient needs the number from its first row on.
 template <int THREADS>
 __device__ __forceinline__ long long count_rows(const int *targets, long long rows, double *scratch)
@@ -50,90 +61,340 @@ __device__ __forceinline__ long long count_rows(const int *targets, long long ro
     return static_cast<long long>(block_sum_f64<THREADS>(mine, scratch));
 }
 
-// What a block knows of its segment of a row; with several blocks a row each sends its own to all.
-struct alignas(16) SegmentSums
+// What the parts of a row tell each other, an array a quantity: n_warps places for the sweeping warps of the cluster,
+// `blocks` for its blocks. Every block of a cluster holds all of them.
+struct RowSums
 {
-    float m_u;              // maximum of the columns that are neither listed nor the label
-    float m_l;              // maximum of the listed ones
-    float z_y;              // the label's logit, -inf where it is in another segment
-    int label_listed;
-    double s_t, s_1;        // sums over the first kind, relative to m_u, at the temperature and at 1
-    double l_t, l_1;        // sums over the listed, relative to m_l
-    double part, own;       // sum p (log p - (z - m_l) / T), sum p
-};
+    double *l_t, *l_1;      // sums over the listed columns, at the temperature and at 1, relative to m_l
+    double *part, *own;     // sum w (log w - (z - m_l) / T) and sum w over them; w: the teacher's masses before the norm
+    float *m_l, *z_y;       // maximum of the listed ones; the label's logit, -inf where it is in another segment
+    float *m_u, *s_t, *s_1; // a warp's maximum and sums of the columns neither listed nor the label
 
-// What the gradient needs of a whole row.
-struct RowFactors
-{
-    float m_u, f_t, f_1;    // a column that is not listed: e^((z - m_u) / T) f_t + e^(z - m_u) f_1
-    float m;
-    double l_t, l_1;        // a listed one: e^((z - m) / T) l_t + e^(z - m) l_1 - p soft_scale
-    double y;               // what the label's column has besides
-    double label;           // the label's column where it is not listed
+    __device__ __forceinline__ RowSums(char *base, int blocks, int n_warps)
+    {
+        l_t = reinterpret_cast<double *>(base);
+        l_1 = l_t + blocks;
+        part = l_1 + blocks;
+        own = part + blocks;
+        m_l = reinterpret_cast<float *>(own + blocks);
+        z_y = m_l + blocks;
+        m_u = z_y + blocks;
+        s_t = m_u + n_warps;
+        s_1 = s_t + n_warps;
+    }
 };
+__host__ __device__ inline int row_sums_bytes(int blocks, int n_warps)
+{
+    return blocks * static_cast<int>(4 * sizeof(double) + 2 * sizeof(float)) + n_warps * static_cast<int>(3 * sizeof(float));
+}
 
 // e^((from - to) f), 0 from -inf
 __device__ __forceinline__ double shifted(float from, float to, double f)
 {
     return from == -INFINITY ? 0.0 : from == to ? 1.0 : exp((static_cast<double>(from) - static_cast<double>(to)) * f);
 }
+__device__ __forceinline__ float shifted_fast(float from, float to, float c)
+{
+    return from == -INFINITY ? 0.0f : exp2_fast((from - to) * c);
+}
 
-// A cluster a row, the row in its shared memory between the sweeps. Barriers of a block and row: the row has
-// arrived; listed columns are taken out; maximum; sums; factors; the gradient is out.
-template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_rows_kernel(const DistillArgs a, const RowPlan plan)
+// Sum over the first n lanes (a power of two), in every lane.
+template <typename V>
+__device__ __forceinline__ V sum_lanes(V v, int n)
+{
+    for (int offset = n >> 1; offset > 0; offset >>= 1)
+    {
+        v += __shfl_xor_sync(0xffffffffu, v, offset);
+    }
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+
+// The sweeps of the segment. TWO: two softmaxes of a row, at the temperature and at 1.
+template <bool TWO, typename T, int THREADS>
+__device__ __forceinline__ void sweep_sums(const RowTile<T, THREADS> &tile, float ref, float c_t, float c_1, float *s_t, float *s_1)
+{
+    constexpr int PAIRS = Vec16<T>::N / 2;
+    const float2 minus_ref = make_float2(-ref, -ref), c_t2 = make_float2(c_t, c_t), c_12 = make_float2(c_1, c_1);
+    float2 sum_t = make_float2(0.0f, 0.0f), sum_1 = make_float2(0.0f, 0.0f);
+    for (int i = threadIdx.x; i < tile.vecs; i += THREADS)
+    {
+        float2 f[PAIRS];
+        unpack(tile.vec(i), f);
+#pragma unroll
+        for (int q = 0; q < PAIRS; q++)
+        {
+            const float2 d = add2(f[q], minus_ref);
+            const float2 x = mul2(d, c_t2);
+            sum_t = add2(sum_t, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+            if (TWO)
+            {
+                const float2 x1 = mul2(d, c_12);
+                sum_1 = add2(sum_1, make_float2(exp2_fast(x1.x), exp2_fast(x1.y)));
+            }
+        }
+    }
+    *s_t = warp_sum_f32(sum_t.x + sum_t.y);
+    *s_1 = TWO ? warp_sum_f32(sum_1.x + sum_1.y) : *s_t;
+}
+
+template <bool TWO, typename T, int THREADS>
+__device__ __forceinline__ Vec16<T> gradient_of(const RowTile<T, THREADS> &tile, int i, float ref, float c_t, float c_1,
+                                                float f_t, float f_1)
+{
+    constexpr int PAIRS = Vec16<T>::N / 2;
+    const float2 minus_ref = make_float2(-ref, -ref), c_t2 = make_float2(c_t, c_t), c_12 = make_float2(c_1, c_1);
+    const float2 f_t2 = make_float2(f_t, f_t), f_12 = make_float2(f_1, f_1);
+    float2 f[PAIRS];
+    unpack(tile.vec(i), f);
+#pragma unroll
+    for (int q = 0; q < PAIRS; q++)
+    {
+        const float2 d = add2(f[q], minus_ref);
+        const float2 x = mul2(d, c_t2);
+        f[q] = mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), f_t2);
+        if (TWO)
+        {
+            const float2 x1 = mul2(d, c_12);
+            f[q] = fma2(make_float2(exp2_fast(x1.x), exp2_fast(x1.y)), f_12, f[q]);
+        }
+    }
+    Vec16<T> g;
+    pack(g, f);
+    return g;
+}
+
+// Named barriers: 1 among the sweeping threads, 2 for the block where its two parts come from different code.
+template <int THREADS>
+__device__ __forceinline__ void sweep_barrier()
+{
+    asm volatile("bar.sync 1, %0;" : : "n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void both_barrier()
+{
+    asm volatile("bar.sync 2, %0;" : : "n"(THREADS) : "memory");
+}
+
+// The gradient of the segment's columns; the listed ones and the label's are written over afterwards.
+template <bool TWO, typename T, int THREADS>
+__device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, T *out, float ref, float c_t, float c_1, float f_t,
+                                               float f_1)
+{
+    constexpr int N = Vec16<T>::N;
+    const int tid = threadIdx.x;
+    char *dst = reinterpret_cast<char *>(out + tile.first) - tile.lead * sizeof(T);
+    if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0)
+    {
+        // the row starts as far from a 16-byte boundary as the logits' row: whole vectors, then the two ends
+        const int whole_first = tile.lead > 0 ? 1 : 0, whole_end = (tile.lead + tile.held) / N;
+        for (int i = whole_first + tid; i < whole_end; i += THREADS)
+        {
+            *reinterpret_cast<uint4 *>(dst + 16ll * i) = gradient_of<TWO>(tile, i, ref, c_t, c_1, f_t, f_1).w;
+        }
+        const bool front = tid == 0 && tile.lead > 0;
+        const bool back = tid == 1 && whole_end < tile.vecs && whole_end >= whole_first;
+        if (front || back)
+        {
+            const int i = front ? 0 : whole_end;
+            const Vec16<T> g = gradient_of<TWO>(tile, i, ref, c_t, c_1, f_t, f_1);
+            const T *e = reinterpret_cast<const T *>(&g);
+            for (int q = 0; q < N; q++)
+            {
+                if (i * N + q >= tile.lead && i * N + q < tile.lead + tile.held)
+                {
+                    reinterpret_cast<T *>(dst)[i * N + q] = e[q];
+                }
+            }
+        }
+        return;
+    }
+    for (int i = tid; i < tile.vecs; i += THREADS)
+    {
+        reinterpret_cast<Vec16<T> *>(tile.buf)[i] = gradient_of<TWO>(tile, i, ref, c_t, c_1, f_t, f_1);
+    }
+    sweep_barrier<THREADS>();
+    for (int i = tid; i < tile.held; i += THREADS)
+    {
+        out[tile.first + i] = reinterpret_cast<const T *>(tile.buf)[tile.lead + i];
+    }
+}
+
+// A cluster a row, the row in its shared memory between the sweeps. A block has SWEEP threads that sweep the segment
+// and one more warp for what there is one of a row: the record, the factors, the loss, the listed columns. That warp
+// works while the others sweep, so its fp64 chains are off the row's path, and they are issued once a block and not once
+// a warp (done by every warp they were two thirds of all instructions). Barriers of a block and row:
+//     arrived   the row is in shared memory
+//     marked    the listed columns and the label have been taken out of it
+//     summed    (the cluster's) every warp's sums are with every block
+//     factors   the row's factors are known
+//     written   the gradient is out; the row's place may be filled again
+template <typename T, int SWEEP>
+__global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(const DistillArgs a, const RowPlan plan)
 {
     namespace cg = cooperative_groups;
-    using Tile = RowTile<T, THREADS>;
-    constexpr int N = Tile::N, PAIRS = N / 2, WARPS = THREADS / 32;
+    using Tile = RowTile<T, SWEEP>;
+    constexpr int THREADS = SWEEP + 32, WARPS = SWEEP / 32;     // WARPS: those that sweep
     extern __shared__ __align__(16) char dynamic[];
-    __shared__ SegmentSums slots[2][MAX_CLUSTER];
-    __shared__ RowFactors factors;
-    __shared__ double scratch[WARPS];
-    __shared__ double warp_sums[WARPS][8];
-    __shared__ float2 warp_max[WARPS];
-    __shared__ float label_logit;
-    __shared__ int label_listed, last_block;
+    __shared__ double scratch[THREADS / 32];
+    __shared__ float shared_ref, shared_f_t, shared_f_1;
+    __shared__ int last_block;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool sweeps = warp < WARPS;
     const cg::cluster_group cluster = cg::this_cluster();
     const int blocks = plan.cluster, rank = blocks > 1 ? static_cast<int>(cluster.block_rank()) : 0;
+    const int n_warps = blocks * WARPS;
     const float inf = INFINITY;
 
+    // dynamic shared memory: the segment; two rows' sums; two rows' listed columns of the segment (mass, its logarithm,
+    // logit, column); a table that finds columns listed twice
     const size_t tile_bytes = (static_cast<size_t>(plan.segment) * sizeof(T) + 31) & ~static_cast<size_t>(15);
+    const int sums_bytes = (row_sums_bytes(blocks, n_warps) + 7) & ~7;
     Tile tile;
     tile.buf = dynamic;
-    double *rec_lp = reinterpret_cast<double *>(dynamic + tile_bytes);      // log p, p, logit and column of what is listed
-    double *rec_p = rec_lp + a.k;
-    float *rec_z = reinterpret_cast<float *>(rec_p + a.k);
-    int *rec_col = reinterpret_cast<int *>(rec_z + a.k);
-    unsigned int *marked = reinterpret_cast<unsigned int *>(rec_col + a.k); // a bit a column of the segment
-    for (int w = tid; w < plan.segment / 32; w += THREADS)
-    {
-        marked[w] = 0u;
-    }
+    char *const sums = dynamic + tile_bytes;
+    double *const rec_w0 = reinterpret_cast<double *>(sums + 2 * sums_bytes);
+    double *const rec_lw0 = rec_w0 + 2 * a.k;
+    float *const rec_z0 = reinterpret_cast<float *>(rec_lw0 + 2 * a.k);
+    int *const rec_col0 = reinterpret_cast<int *>(rec_z0 + 2 * a.k);
+    int *const table = rec_col0 + 2 * a.k;
+    const int table_mask = distill_table(a.k) - 1;
 
     const bool hard = a.hard != 0.0;
-    const double inv_t = a.k > 0 ? 1.0 / a.temperature : 1.0;      // the label's softmax alone is at 1
-    const bool two = hard && a.k > 0 && a.temperature != 1.0;   // two softmaxes of a row
+    const double inv_t = a.k > 0 ? 1.0 / a.temperature : 1.0;       // the label's softmax alone is at 1
+    const bool two = hard && a.k > 0 && a.temperature != 1.0;       // two softmaxes of a row
     const double log2e = 1.4426950408889634;
     const float c_t = static_cast<float>(log2e * inv_t), c_1 = static_cast<float>(log2e);
-    const int segment_first = rank * plan.segment;
+    const int first = rank * plan.segment;
+    const int valid = max(0, min(plan.segment, a.vocab - first)), held = max(0, min(plan.segment, a.cols - first));
     const long long clusters = gridDim.x / blocks;
-    auto row_of = [&](long long row) { return static_cast<const T *>(a.logits) + row * a.ld; };
-    auto label_of = [&](long long row) { return a.targets != nullptr ? __ldg(&a.targets[row]) : 0; };
+    auto label_of = [&](long long row) { return row >= a.rows ? -1 : a.targets != nullptr ? __ldg(&a.targets[row]) : 0; };
+    auto start = [&](long long row) {
+        if (sweeps)
+        {
+            tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.cols);
+        }
+    };
 
     long long row = blockIdx.x / blocks;
-    bool started = false;
-    if (row < a.rows && label_of(row) >= 0)
+    int y = label_of(row);
+    bool started = y >= 0;
+    if (started)
     {
-        tile.start(row_of(row), segment_first, plan.segment, a.vocab, a.cols);
-        started = true;
+        start(row);
     }
     const long long n_valid = count_rows<THREADS>(a.targets, a.rows, scratch);
     const double grad_scale = static_cast<double>(a.st->loss_scale) / static_cast<double>(n_valid > 0 ? n_valid : 1);
-    const double soft_scale = a.k > 0 ? grad_scale * a.soft * inv_t : 0.0;
-    const double hard_scale = hard ? grad_scale * a.hard : 0.0;
+    const float soft_scale = a.k > 0 ? static_cast<float>(grad_scale * a.soft * inv_t) : 0.0f;
+    const float hard_scale = hard ? static_cast<float>(grad_scale * a.hard) : 0.0f;
+    for (int i = tid; i <= table_mask; i += THREADS)
+    {
+        table[i] = -1;
+    }
     __syncthreads();
+
+    // the record of a row into rec[parity], by the last warp: its columns in this segment, in the record's order. Masses
+    // are w = e^(t / T - lse), or, before the norm that the cluster works out, e^((t - max) / T).
+    struct Record
+    {
+        int n;                  // listed columns of this segment
+        bool label_listed;      // anywhere in the row
+        double own;             // sum of their masses; NaN if a column is beyond the vocabulary
+    };
+    auto read_record = [&](long long at, int label, int parity) {
+        Record r = {0, false, 0.0};
+        double *w_of = rec_w0 + parity * a.k, *lw_of = rec_lw0 + parity * a.k;
+        float *z_of = rec_z0 + parity * a.k;
+        int *col_of = rec_col0 + parity * a.k;
+        const long long base = at * a.k;
+        double shift = 0.0;
+        if (a.lse != nullptr)
+        {
+            shift = __ldg(&a.lse[at]);
+        }
+        else
+        {
+            float t_max = -inf;
+            for (int j = lane; j < a.k; j += 32)
+            {
+                if (__ldg(&a.indices[base + j]) >= 0)
+                {
+                    t_max = max_nan(t_max, load_typed(a.values, a.value_dtype, base + j));
+                }
+            }
+            t_max = warp_max_nan(t_max);
+            shift = t_max == -inf ? 0.0 : t_max * inv_t;
+        }
+        bool beyond = false, twice = false;
+        for (int j0 = 0; j0 < a.k; j0 += 32)
+        {
+            const int j = j0 + lane;
+            const int v = j < a.k ? __ldg(&a.indices[base + j]) : -1;
+            beyond = beyond || v >= a.vocab;
+            r.label_listed = r.label_listed || (hard && v == label);
+            const bool mine = v >= first && v < first + valid;
+            const unsigned int ballot = __ballot_sync(0xffffffffu, mine);
+            if (mine)
+            {
+                const int to = r.n + __popc(ballot & ((1u << lane) - 1u));
+                const double lw = load_typed(a.values, a.value_dtype, base + j) * inv_t - shift, w = exp(lw);
+                lw_of[to] = lw;
+                w_of[to] = w;
+                col_of[to] = v;
+                r.own += w;
+                for (int p = v & table_mask;; p = (p + 1) & table_mask)        // twice as many places as columns
+                {
+                    const int there = atomicCAS(&table[p], -1, v);
+                    if (there == -1 || there == v)
+                    {
+                        twice = twice || there == v;
+                        break;
+                    }
+                }
+            }
+            r.n += __popc(ballot);
+        }
+        r.label_listed = __any_sync(0xffffffffu, r.label_listed);
+        __syncwarp();
+        for (int i = lane; i <= table_mask; i += 32)
+        {
+            table[i] = -1;
+        }
+        if (__any_sync(0xffffffffu, twice))
+        {
+            // a column listed more than once keeps its first place, with all its mass
+            for (int i = lane; i < r.n; i += 32)
+            {
+                bool is_first = true;
+                double w = 0.0;
+                for (int q = 0; q < r.n; q++)
+                {
+                    is_first = is_first && !(q < i && col_of[q] == col_of[i]);
+                    w += col_of[q] == col_of[i] ? w_of[q] : 0.0;
+                }
+                z_of[i] = is_first ? 1.0f : 0.0f;
+                lw_of[i] = log(w);
+            }
+            __syncwarp();
+            for (int i = lane; i < r.n; i += 32)
+            {
+                w_of[i] = exp(lw_of[i]);
+                col_of[i] = z_of[i] != 0.0f ? col_of[i] : -1;
+            }
+        }
+        __syncwarp();
+        r.own = warp_sum_f64(r.own);
+        if (__any_sync(0xffffffffu, beyond))
+        {
+            r.own = nan("");
+        }
+        return r;
+    };
+
+    Record record = {0, false, 0.0};
+    if (!sweeps && y >= 0)
+    {
+        record = read_record(row, y, 0);
+    }
     if (blocks > 1)
     {
         cluster.sync();                         // every block of the cluster runs before one writes to another
@@ -142,418 +403,296 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_rows_kernel(c
     for (int parity = 0; row < a.rows; row += clusters)
     {
         T *out = a.dlogits != nullptr ? static_cast<T *>(a.dlogits) + row * a.dld : nullptr;
-        const int y = label_of(row);
+        const int next_y = label_of(row + clusters);
         if (y < 0)
         {
-            const int held = max(0, min(plan.segment, a.cols - segment_first));
             for (int i = tid; out != nullptr && i < held; i += THREADS)
             {
-                out[segment_first + i] = from_float<T>(0.0f);
+                out[first + i] = from_float<T>(0.0f);
             }
             if (rank == 0 && tid == 0)
             {
                 a.row_loss[row] = 0.0f;
             }
+            if (!sweeps && next_y >= 0)
+            {
+                record = read_record(row + clusters, next_y, parity);
+            }
+            y = next_y;
             started = false;
             continue;
         }
         if (!started)
         {
-            tile.start(row_of(row), segment_first, plan.segment, a.vocab, a.cols);
+            start(row);
         }
         const bool label_in = hard && y < a.vocab;
+        char *const place = sums + parity * sums_bytes;
+        double *const rec_w = rec_w0 + parity * a.k, *const rec_lw = rec_lw0 + parity * a.k;
+        float *const rec_z = rec_z0 + parity * a.k;
+        int *const rec_col = rec_col0 + parity * a.k;
+        if (sweeps)
+        {
+            copy_async_wait();
+        }
+        __syncthreads();                        // arrived
 
-        // the record, while the row is on its way
-        bool twice = false;
-        double norm_max = 0.0, log_norm = 0.0;
-        if (a.lse == nullptr && a.k > 0)
+        float m_l = -inf, z_y = -inf;
+        if (!sweeps)
         {
-            float t_max = -inf;
-            for (int j = tid; j < a.k; j += THREADS)
+            // where column v of this segment is: the tile's own reckoning, which the sweeping threads hold
+            const uintptr_t src = reinterpret_cast<uintptr_t>(static_cast<const T *>(a.logits) + row * a.ld + first);
+            T *const e = reinterpret_cast<T *>(dynamic + (src & 15)) - first;
+            for (int i = lane; i < record.n; i += 32)
             {
-                if (a.indices[row * a.k + j] >= 0)
+                const int v = rec_col[i];
+                if (v >= 0)
                 {
-                    t_max = max_nan(t_max, load_typed(a.values, a.value_dtype, row * a.k + j));
+                    const float z = to_float(e[v]);
+                    e[v] = minus_infinity<T>();
+                    rec_z[i] = z;
+                    m_l = max_nan(m_l, z);
+                    z_y = hard && v == y ? z : z_y;
                 }
             }
-            t_max = block_max_nan<THREADS>(t_max, scratch);
-            norm_max = t_max == -inf ? 0.0 : t_max * inv_t;
-            double sum = 0.0;
-            for (int j = tid; j < a.k; j += THREADS)
+            if (lane == 0 && label_in && !record.label_listed && y >= first && y < first + valid)
             {
-                if (a.indices[row * a.k + j] >= 0)
-                {
-                    sum += exp(load_typed(a.values, a.value_dtype, row * a.k + j) * inv_t - norm_max);
-                }
-            }
-            sum = block_sum_f64<THREADS>(sum, scratch);
-            log_norm = sum == 0.0 ? 0.0 : log(sum);
-        }
-        else if (a.lse != nullptr)
-        {
-            log_norm = a.lse[row];
-        }
-        double mass = 0.0;
-        for (int j = tid; j < a.k; j += THREADS)
-        {
-            const int v = a.indices[row * a.k + j];
-            const bool fits = v >= 0 && v < a.vocab;
-            const double lp = load_typed(a.values, a.value_dtype, row * a.k + j) * inv_t - norm_max - log_norm;
-            const double p = fits ? exp(lp) : v < 0 ? 0.0 : nan("");    // beyond the vocabulary: the row is NaN
-            mass += p;
-            rec_lp[j] = lp;
-            rec_p[j] = p;
-            rec_col[j] = fits ? v : -1;
-            if (fits && tile.holds(v))
-            {
-                const int at = v - segment_first;
-                twice = twice || (atomicOr(&marked[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u) != 0;
+                z_y = to_float(e[y]);
+                e[y] = minus_infinity<T>();
             }
         }
-        if (tid == 0)
-        {
-            label_logit = -inf;
-            label_listed = 0;
-        }
-        copy_async_wait();
-        if (__syncthreads_or(twice) != 0)
-        {
-            // a column listed more than once keeps its first place, with all its mass
-            for (int j = tid; j < a.k; j += THREADS)
-            {
-                const int v = rec_col[j];
-                bool first = true;
-                double p = 0.0;
-                for (int i = 0; v >= 0 && i < a.k; i++)
-                {
-                    first = first && !(i < j && rec_col[i] == v);
-                    p += rec_col[i] == v ? rec_p[i] : 0.0;
-                }
-                rec_z[j] = first ? 1.0f : 0.0f;
-                rec_lp[j] = log(p);
-            }
-            __syncthreads();
-            for (int j = tid; j < a.k; j += THREADS)
-            {
-                if (rec_col[j] >= 0)
-                {
-                    rec_p[j] = exp(rec_lp[j]);
-                    rec_col[j] = rec_z[j] != 0.0f ? rec_col[j] : -1;
-                }
-            }
-        }
+        __syncthreads();                        // marked
 
-        // take the listed columns and the label out of the row
-        float m_l = -inf;
-        for (int j = tid; j < a.k; j += THREADS)
+        if (sweeps)
         {
-            const int v = rec_col[j];
-            if (tile.holds(v))
-            {
-                const float z = to_float(*tile.at(v));
-                *tile.at(v) = minus_infinity<T>();
-                rec_z[j] = z;
-                m_l = max_nan(m_l, z);
-                if (label_in && v == y)
-                {
-                    label_logit = z;
-                    label_listed = 1;
-                }
-            }
-        }
-        if (tid == 0 && label_in && tile.holds(y))
-        {
-            const int at = y - segment_first;
-            if ((marked[at >> 5] >> (at & 31) & 1u) == 0)
-            {
-                label_logit = to_float(*tile.at(y));
-                *tile.at(y) = minus_infinity<T>();
-            }
-        }
-        __syncthreads();
-        for (int j = tid; j < a.k; j += THREADS)
-        {
-            if (tile.holds(rec_col[j]))
-            {
-                marked[(rec_col[j] - segment_first) >> 5] = 0u;
-            }
-        }
-
-        // maxima
-        Vec16<T> best;
-        {
+            // sums of this warp's share, relative to its own maximum
+            Vec16<T> best;
             const T low = minus_infinity<T>();
             T *e = reinterpret_cast<T *>(&best);
 #pragma unroll
-            for (int i = 0; i < N; i++)
+            for (int i = 0; i < Vec16<T>::N; i++)
             {
                 e[i] = low;
             }
-        }
-        for (int i = tid; i < tile.vecs; i += THREADS)
-        {
-            max_into(best, tile.vec(i));
-        }
-        const float m_warp = warp_max_nan(max_of(best));
-        m_l = warp_max_nan(m_l);
-        if (lane == 0)
-        {
-            warp_max[warp] = make_float2(m_warp, m_l);
-        }
-        __syncthreads();
-        float m_u = -inf;
-        m_l = -inf;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++)
-        {
-            m_u = max_nan(m_u, warp_max[w].x);
-            m_l = max_nan(m_l, warp_max[w].y);
-        }
-
-        // sums, relative to them
-        {
-            const float ref = m_u == -inf ? 0.0f : m_u;         // nothing but -inf: every term is 0
-            const float2 minus_ref = make_float2(-ref, -ref), c_t2 = make_float2(c_t, c_t), c_12 = make_float2(c_1, c_1);
-            float2 sum_t = make_float2(0.0f, 0.0f), sum_1 = make_float2(0.0f, 0.0f);
-            for (int i = tid; i < tile.vecs; i += THREADS)
+            for (int i = tid; i < tile.vecs; i += SWEEP)
             {
-                float2 f[PAIRS];
-                unpack(tile.vec(i), f);
-#pragma unroll
-                for (int q = 0; q < PAIRS; q++)
-                {
-                    const float2 d = add2(f[q], minus_ref);
-                    const float2 x = mul2(d, c_t2);
-                    sum_t = add2(sum_t, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
-                    if (two)
-                    {
-                        const float2 x1 = mul2(d, c_12);
-                        sum_1 = add2(sum_1, make_float2(exp2_fast(x1.x), exp2_fast(x1.y)));
-                    }
-                }
+                max_into(best, tile.vec(i));
             }
-            double l_t = 0.0, l_1 = 0.0, part = 0.0, own = 0.0;
-            const double ref_l = m_l == -inf ? 0.0 : m_l;
-            for (int j = tid; j < a.k; j += THREADS)
+            const float m_u = warp_max_nan(max_of(best));
+            const float ref = m_u == -inf ? 0.0f : m_u;         // nothing but -inf: every term is 0
+            float s_t, s_1;
+            if (two)
             {
-                if (tile.holds(rec_col[j]))
+                sweep_sums<true>(tile, ref, c_t, c_1, &s_t, &s_1);
+            }
+            else
+            {
+                sweep_sums<false>(tile, ref, c_t, c_1, &s_t, &s_1);
+            }
+            if (lane < blocks)
+            {
+                const RowSums to(blocks > 1 ? cluster.map_shared_rank(place, lane) : place, blocks, n_warps);
+                to.m_u[rank * WARPS + warp] = m_u;
+                to.s_t[rank * WARPS + warp] = s_t;
+                to.s_1[rank * WARPS + warp] = s_1;
+            }
+        }
+        else
+        {
+            m_l = warp_max_nan(m_l);
+            z_y = warp_max_nan(z_y);
+            const double ref_l = m_l == -inf ? 0.0 : m_l;
+            double l_t = 0.0, l_1 = 0.0, part = 0.0;
+            for (int i = lane; i < record.n; i += 32)
+            {
+                if (rec_col[i] >= 0)
                 {
-                    const double d = rec_z[j] - ref_l, p = rec_p[j];
+                    const double d = rec_z[i] - ref_l, w = rec_w[i];
                     l_t += exp(d * inv_t);
                     l_1 += two ? exp(d) : 0.0;
-                    part += p != 0.0 ? p * (rec_lp[j] - d * inv_t) : 0.0;
-                    own += p;
+                    part += w != 0.0 ? w * (rec_lw[i] - d * inv_t) : 0.0;
                 }
             }
-            const float s_t = warp_sum_f32(sum_t.x + sum_t.y), s_1 = warp_sum_f32(sum_1.x + sum_1.y);
-            if (warp * 32 < a.k)                // the others have no listed columns
+            if (record.n > 0)
             {
                 l_t = warp_sum_f64(l_t);
-                l_1 = warp_sum_f64(l_1);
+                l_1 = two ? warp_sum_f64(l_1) : l_t;
                 part = warp_sum_f64(part);
-                own = warp_sum_f64(own);
-                mass = warp_sum_f64(mass);
             }
-            if (lane == 0)
+            if (lane < blocks)
             {
-                double *w = warp_sums[warp];
-                w[0] = s_t;
-                w[1] = s_1;
-                w[2] = l_t;
-                w[3] = l_1;
-                w[4] = part;
-                w[5] = own;
-                w[6] = mass;
-            }
-        }
-        __syncthreads();
-
-        // the blocks of the cluster exchange theirs; the first warp of each works out the row's factors
-        double others = 0.0, o_in_all = 0.0, total = 0.0, total_1 = 0.0, part = 0.0, rest = 0.0, whole = 0.0, d_y = 0.0;
-        float m = 0.0f, m_o = 0.0f;
-        if (warp == 0)
-        {
-            double sum = 0.0;
-            if (lane < 7)
-            {
-                for (int w = 0; w < WARPS; w++)
-                {
-                    sum += warp_sums[w][lane];
-                }
-            }
-            SegmentSums mine;
-            mine.m_u = m_u;
-            mine.m_l = m_l;
-            mine.z_y = label_logit;
-            mine.label_listed = label_listed;
-            mine.s_t = __shfl_sync(0xffffffffu, sum, 0);
-            mine.s_1 = __shfl_sync(0xffffffffu, sum, 1);
-            mine.l_t = __shfl_sync(0xffffffffu, sum, 2);
-            mine.l_1 = __shfl_sync(0xffffffffu, sum, 3);
-            mine.part = __shfl_sync(0xffffffffu, sum, 4);
-            mine.own = __shfl_sync(0xffffffffu, sum, 5);
-            mass = __shfl_sync(0xffffffffu, sum, 6);
-            if (blocks == 1)
-            {
-                slots[parity][0] = mine;        // every lane writes the same
-            }
-            else if (lane < blocks)
-            {
-                *cluster.map_shared_rank(&slots[parity][rank], lane) = mine;
+                const RowSums to(blocks > 1 ? cluster.map_shared_rank(place, lane) : place, blocks, n_warps);
+                to.l_t[rank] = l_t;
+                to.l_1[rank] = l_1;
+                to.part[rank] = part;
+                to.own[rank] = record.own;
+                to.m_l[rank] = m_l;
+                to.z_y[rank] = z_y;
             }
         }
         if (blocks > 1)
         {
-            cluster.sync();
+            cluster.sync();                     // summed
         }
-        if (warp == 0)
+        else
         {
-            __syncwarp();
-            SegmentSums s = {-inf, -inf, -inf, 0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-            if (lane < blocks)
-            {
-                s = slots[parity][lane];
-            }
-            const float all_u = warp_max_nan(s.m_u), all_l = warp_max_nan(s.m_l), z_y = warp_max_nan(s.z_y);
-            const bool listed = __any_sync(0xffffffffu, s.label_listed != 0);
-            m_o = listed ? all_u : max_nan(all_u, z_y);         // of the columns not listed
-            m = max_nan(m_o, all_l);
-            const double u_t = warp_sum_f64(s.s_t * shifted(s.m_u, all_u, inv_t));
-            const double u_1 = two ? warp_sum_f64(s.s_1 * shifted(s.m_u, all_u, 1.0)) : u_t;
-            const double listed_t = warp_sum_f64(s.l_t * shifted(s.m_l, m, inv_t));
-            const double listed_1 = two ? warp_sum_f64(s.l_1 * shifted(s.m_l, m, 1.0)) : listed_t;
-            const double ref_l = s.m_l == -inf ? 0.0 : s.m_l;
-            part = warp_sum_f64(s.part + (s.own != 0.0 ? s.own * (m - ref_l) * inv_t : 0.0));
-            const double u_in_o = shifted(all_u, m_o, inv_t), y_in_o = listed ? 0.0 : shifted(z_y, m_o, inv_t);
-            others = u_t * u_in_o + y_in_o;
-            o_in_all = shifted(m_o, m, inv_t);
-            total = others * o_in_all + listed_t;
-            const double u_in_all_1 = two ? shifted(all_u, m, 1.0) : u_in_o * o_in_all;
-            const double y_in_all_1 = two ? shifted(z_y, m, 1.0) : shifted(z_y, m, inv_t);
-            total_1 = u_1 * u_in_all_1 + listed_1 + (listed ? 0.0 : y_in_all_1);
-            rest = a.lse != nullptr && others > 0.0 ? fmax(0.0, 1.0 - mass) : 0.0;
-            whole = mass + rest;
-            d_y = static_cast<double>(z_y) - static_cast<double>(m);
-            const double poison = !isfinite(m) || (hard && !label_in) ? nan("") : 0.0;
-            part += poison;
-            const double per_o = whole * o_in_all / total - (rest > 0.0 ? rest / others : 0.0);     // of e^(x - m_o)
-            if (lane == 0)
-            {
-                const double f_t = soft_scale * per_o * u_in_o + poison;
-                const double f_1 = hard ? hard_scale * u_in_all_1 / total_1 : 0.0;
-                factors.m_u = all_u == -inf ? 0.0f : all_u;
-                factors.f_t = static_cast<float>(two ? f_t : f_t + f_1);
-                factors.f_1 = static_cast<float>(f_1);
-                factors.m = m;
-                factors.l_t = soft_scale * whole / total + poison + (two || !hard ? 0.0 : hard_scale / total_1);
-                factors.l_1 = two ? hard_scale / total_1 : 0.0;
-                factors.y = hard_scale;
-                factors.label = soft_scale * per_o * y_in_o + hard_scale * (y_in_all_1 - total_1) / total_1 + poison;
-            }
+            __syncthreads();
         }
-        parity ^= 1;
-        __syncthreads();
 
-        // gradient
-        if (out != nullptr && tile.vecs > 0)
+        if (sweeps)
         {
-            const float ref = factors.m_u, f_t = factors.f_t, f_1 = factors.f_1;
-            const float2 minus_ref = make_float2(-ref, -ref), c_t2 = make_float2(c_t, c_t), c_12 = make_float2(c_1, c_1);
-            const float2 f_t2 = make_float2(f_t, f_t), f_12 = make_float2(f_1, f_1);
-            char *dst = reinterpret_cast<char *>(out + segment_first) - tile.lead * sizeof(T);
-            const bool same = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;                 // the row starts as far from a boundary as the logits'
-            const int whole_first = tile.lead > 0 ? 1 : 0, whole_end = (tile.lead + tile.held) / N;
-            for (int i = tid; i < tile.vecs; i += THREADS)
+            both_barrier<THREADS>();            // factors
+            if (out != nullptr && tile.vecs > 0)
             {
-                float2 f[PAIRS];
-                unpack(tile.vec(i), f);
-#pragma unroll
-                for (int q = 0; q < PAIRS; q++)
+                if (two)
                 {
-                    const float2 d = add2(f[q], minus_ref);
-                    const float2 x = mul2(d, c_t2);
-                    f[q] = mul2(make_float2(exp2_fast(x.x), exp2_fast(x.y)), f_t2);
-                    if (two)
-                    {
-                        const float2 x1 = mul2(d, c_12);
-                        f[q] = fma2(make_float2(exp2_fast(x1.x), exp2_fast(x1.y)), f_12, f[q]);
-                    }
-                }
-                Vec16<T> g;
-                pack(g, f);
-                if (same && i >= whole_first && i < whole_end)
-                {
-                    *reinterpret_cast<uint4 *>(dst + 16ll * i) = g.w;
-                }
-                else if (same)
-                {
-                    const T *e = reinterpret_cast<const T *>(&g);
-#pragma unroll
-                    for (int q = 0; q < N; q++)
-                    {
-                        if (i * N + q >= tile.lead && i * N + q < tile.lead + tile.held)
-                        {
-                            reinterpret_cast<T *>(dst)[i * N + q] = e[q];
-                        }
-                    }
+                    sweep_gradient<true>(tile, out, shared_ref, c_t, c_1, shared_f_t, shared_f_1);
                 }
                 else
                 {
-                    reinterpret_cast<Vec16<T> *>(tile.buf)[i] = g;
+                    sweep_gradient<false>(tile, out, shared_ref, c_t, c_1, shared_f_t, shared_f_1);
                 }
             }
-            if (!same)
+            both_barrier<THREADS>();            // written
+            started = next_y >= 0;
+            if (started)
             {
-                __syncthreads();
-                for (int i = tid; i < tile.held; i += THREADS)
-                {
-                    out[segment_first + i] = reinterpret_cast<const T *>(tile.buf)[tile.lead + i];
-                }
+                start(row + clusters);
             }
         }
-        __syncthreads();
+        else
+        {
+            // the row's factors; fp32 does for the gradient
+            const RowSums all(place, blocks, n_warps);
+            const bool listed_y = record.label_listed;
+            float all_u = -inf;
+            for (int i = lane; i < n_warps; i += 32)
+            {
+                all_u = max_nan(all_u, all.m_u[i]);
+            }
+            const bool is_block = lane < blocks;
+            const float block_l = is_block ? all.m_l[lane] : -inf;
+            const double block_lt = is_block ? all.l_t[lane] : 0.0, block_l1 = is_block ? all.l_1[lane] : 0.0;
+            const double block_own = is_block ? all.own[lane] : 0.0, block_part = is_block ? all.part[lane] : 0.0;
+            all_u = warp_max_nan(all_u);
+            float all_l = block_l;
+            z_y = is_block ? all.z_y[lane] : -inf;
+            for (int offset = blocks >> 1; offset > 0; offset >>= 1)
+            {
+                all_l = max_nan(all_l, __shfl_xor_sync(0xffffffffu, all_l, offset));
+                z_y = max_nan(z_y, __shfl_xor_sync(0xffffffffu, z_y, offset));
+            }
+            all_l = __shfl_sync(0xffffffffu, all_l, 0);
+            z_y = __shfl_sync(0xffffffffu, z_y, 0);
+            const float m_o = listed_y ? all_u : max_nan(all_u, z_y);       // of the columns not listed
+            const float m = max_nan(m_o, all_l);
+            float u_t = 0.0f, u_1 = 0.0f;
+            for (int i = lane; i < n_warps; i += 32)
+            {
+                const float in_u = shifted_fast(all.m_u[i], all_u, c_t);
+                u_t = fmaf(all.s_t[i], in_u, u_t);
+                u_1 += two ? all.s_1[i] * shifted_fast(all.m_u[i], all_u, c_1) : 0.0f;
+            }
+            u_t = warp_sum_f32(u_t);
+            u_1 = two ? warp_sum_f32(u_1) : u_t;
+            const float listed_t = sum_lanes(static_cast<float>(block_lt) * shifted_fast(block_l, m, c_t), blocks);
+            const float listed_1 = two ? sum_lanes(static_cast<float>(block_l1) * shifted_fast(block_l, m, c_1), blocks) : listed_t;
+            const double own = sum_lanes(block_own, blocks);
+            // mass of the listed columns, and what a w is multiplied by
+            const double mass = a.lse != nullptr ? own : own == 0.0 ? 0.0 : own / own;
+            const double norm = a.lse != nullptr || own == 0.0 ? 1.0 : 1.0 / own;
+            const float u_in_o = shifted_fast(all_u, m_o, c_t), y_in_o = listed_y ? 0.0f : shifted_fast(z_y, m_o, c_t);
+            const float others = fmaf(u_t, u_in_o, y_in_o);
+            const float o_in_all = shifted_fast(m_o, m, c_t);
+            const float total = fmaf(others, o_in_all, listed_t);
+            const double rest = a.lse != nullptr && a.k > 0 && others > 0.0f ? fmax(0.0, 1.0 - mass) : 0.0;
+            const float poison = !isfinite(m) || (hard && !label_in) ? NAN : 0.0f;
+            const float whole = static_cast<float>(mass + rest) + poison;
+            const float u_in_all_1 = two ? shifted_fast(all_u, m, c_1) : u_in_o * o_in_all;
+            const float not_y_1 = fmaf(u_1, u_in_all_1, listed_1);          // all but the label, where that is not listed
+            const float total_1 = not_y_1 + (listed_y ? 0.0f : shifted_fast(z_y, m, c_1));
+            const float per_o = whole * o_in_all / total - (rest > 0.0 ? static_cast<float>(rest) / others : 0.0f);
+            const float f_1 = hard ? hard_scale * u_in_all_1 / total_1 : 0.0f;
+            if (lane == 0)
+            {
+                shared_ref = all_u == -inf ? 0.0f : all_u;
+                shared_f_t = soft_scale * per_o * u_in_o + poison + (two ? 0.0f : f_1);
+                shared_f_1 = f_1;
+            }
+            both_barrier<THREADS>();            // factors
 
-        // the next row is on its way while the listed columns and the loss are written
-        const Tile now = tile;
-        started = row + clusters < a.rows && label_of(row + clusters) >= 0;
-        if (started)
-        {
-            tile.start(row_of(row + clusters), segment_first, plan.segment, a.vocab, a.cols);
-        }
-        for (int j = tid; out != nullptr && j < a.k; j += THREADS)
-        {
-            const int v = rec_col[j];
-            if (now.holds(v))
+            // while the gradient is swept: the loss, in fp64, and the next row's record
+            if (rank == 0)
             {
-                const double d = static_cast<double>(rec_z[j]) - static_cast<double>(factors.m);
-                double g = exp(d * inv_t) * factors.l_t - soft_scale * rec_p[j];
-                if (two)
+                double u_t64 = 0.0, u_164 = 0.0;
+                for (int i = lane; i < n_warps; i += 32)
                 {
-                    g += exp(d) * factors.l_1;
+                    const double in_u = shifted(all.m_u[i], all_u, inv_t);
+                    u_t64 += all.s_t[i] * in_u;
+                    u_164 += two ? all.s_1[i] * shifted(all.m_u[i], all_u, 1.0) : 0.0;
                 }
-                out[v] = from_float<T>(static_cast<float>(label_in && v == y ? g - factors.y : g));
+                u_t64 = warp_sum_f64(u_t64);
+                u_164 = two ? warp_sum_f64(u_164) : u_t64;
+                const double listed_t64 = sum_lanes(block_lt * shifted(block_l, m, inv_t), blocks);
+                const double listed_164 = two ? sum_lanes(block_l1 * shifted(block_l, m, 1.0), blocks) : listed_t64;
+                const double ref_l = block_l == -inf ? 0.0 : block_l;
+                const double part = sum_lanes(block_part + (block_own != 0.0 ? block_own * (m - ref_l) * inv_t : 0.0), blocks);
+                const double o = u_t64 * shifted(all_u, m_o, inv_t) + (listed_y ? 0.0 : shifted(z_y, m_o, inv_t));
+                const double s = o * shifted(m_o, m, inv_t) + listed_t64;
+                const double s_1 = u_164 * shifted(all_u, m, two ? 1.0 : inv_t) + listed_164 + (listed_y ? 0.0 : shifted(z_y, m, 1.0));
+                // one logarithm a lane
+                const double of = lane == 0 ? s : lane == 1 ? s_1 : lane == 2 ? o : lane == 3 ? rest : norm;
+                const double log_of = of > 0.0 ? log(of) : 0.0;
+                const double log_s = __shfl_sync(0xffffffffu, log_of, 0), log_s1 = __shfl_sync(0xffffffffu, log_of, 1);
+                const double log_o = __shfl_sync(0xffffffffu, log_of, 2), log_rest = __shfl_sync(0xffffffffu, log_of, 3);
+                const double log_norm = __shfl_sync(0xffffffffu, log_of, 4);
+                if (lane == 0)
+                {
+                    double loss = 0.0;
+                    if (a.k > 0)
+                    {
+                        loss = part * norm + mass * log_norm + (mass + rest) * log_s;
+                        loss += rest > 0.0 ? rest * (log_rest - log_o - (static_cast<double>(m_o) - m) * inv_t) : 0.0;
+                        loss *= a.soft;
+                    }
+                    if (hard)
+                    {
+                        loss += a.hard * (log_s1 - (static_cast<double>(z_y) - m));
+                    }
+                    a.row_loss[row] = static_cast<float>(loss + poison);
+                }
             }
-        }
-        if (out != nullptr && tid == 0 && label_in && now.holds(y) && label_listed == 0)
-        {
-            out[y] = from_float<T>(static_cast<float>(factors.label));
-        }
-        if (rank == 0 && tid == 0)
-        {
-            double loss = part;                 // carries the poison of a row that has gone wrong
-            if (a.k > 0)
+            const int n_listed = record.n;
+            if (next_y >= 0)
             {
-                const double log_o = rest > 0.0 ? log(others) + (static_cast<double>(m_o) - m) * inv_t : 0.0;
-                loss += whole * log(total) + (rest > 0.0 ? rest * (log(rest) - log_o) : 0.0);
-                loss *= a.soft;
+                record = read_record(row + clusters, next_y, parity ^ 1);
             }
-            if (hard)
+            both_barrier<THREADS>();            // written
+
+            // while the next row is on its way: what the gradient's sweep left to this warp
+            const float l_t = soft_scale * whole / total + (hard && !two ? hard_scale / total_1 : 0.0f);
+            const float l_1 = two ? hard_scale / total_1 : 0.0f;
+            for (int i = lane; out != nullptr && i < n_listed; i += 32)
             {
-                loss += a.hard * (log(total_1) - d_y);
+                const int v = rec_col[i];
+                if (v >= 0)
+                {
+                    float g = fmaf(shifted_fast(rec_z[i], m, c_t), l_t, -soft_scale * static_cast<float>(rec_w[i] * norm)) + poison;
+                    if (two)
+                    {
+                        g = fmaf(shifted_fast(rec_z[i], m, c_1), l_1, g);
+                    }
+                    out[v] = from_float<T>(hard && v == y ? g - hard_scale : g);
+                }
             }
-            a.row_loss[row] = static_cast<float>(loss);
+            if (out != nullptr && lane == 0 && label_in && !listed_y && y >= first && y < first + valid)
+            {
+                out[y] = from_float<T>(soft_scale * per_o * y_in_o - hard_scale * (not_y_1 / total_1) + poison);
+            }
+            started = next_y >= 0;
         }
-        __syncthreads();                        // the record's arrays and the label are written again
+        parity ^= 1;
+        y = next_y;
     }
 
     if (!take_last_ticket(&a.ws->distill_ticket, gridDim.x, &last_block))
@@ -573,18 +712,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) distill_rows_kernel(c
     }
 }
 
-template <typename T, int THREADS>
+template <typename T, int SWEEP>
 static int launch_distill(const DistillArgs &a, RowPlan plan, cudaStream_t stream)
 {
-    return launch_rows(distill_rows_kernel<T, THREADS>, a, plan, a.rows, stream);
+    return launch_rows(distill_rows_kernel<T, SWEEP>, a, plan, SWEEP + 32, a.rows, stream);
 }
 
 template <typename T>
 static int launch_distill(const DistillArgs &a, cudaStream_t stream)
 {
-    const int record = a.k * (2 * sizeof(double) + sizeof(float) + sizeof(int));
+    const int record = 2 * a.k * (2 * sizeof(double) + sizeof(float) + sizeof(int)) + distill_table(a.k) * sizeof(int);
     RowPlan plan;
-    const int rc = plan_rows(a.rows, a.cols, sizeof(T), record, &plan);
+    const int rc = plan_rows(
+        a.rows, a.cols, sizeof(T),
+        [&](int blocks, int warps) { return record + 2 * ((row_sums_bytes(blocks, blocks * warps) + 7) & ~7); }, &plan);
     if (rc != B200AMP_OK)
     {
         return rc;

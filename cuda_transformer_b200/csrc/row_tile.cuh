@@ -24,43 +24,45 @@ struct RowPlan
 {
     int cluster;            // blocks a row
     int segment;            // columns a block, a multiple of 64
-    int threads;
+    int threads;            // that sweep; the kernel may have a warp more
     int smem;               // dynamic shared memory of a block
 };
 
-// Cluster and block size for rows of `cols` elements of `size` bytes, with `more` bytes of shared memory
-// besides the segment. B200AMP_ERR_LIMIT where a row does not fit the largest cluster.
-inline int plan_rows(long long rows, int cols, int size, int more, RowPlan *plan)
+// Cluster and block size for rows of `cols` elements of `size` bytes, with more(blocks, sweeping warps a block)
+// bytes of shared memory besides the segment. B200AMP_ERR_LIMIT where a row does not fit the largest cluster.
+template <typename More>
+int plan_rows(long long rows, int cols, int size, More more, RowPlan *plan)
 {
     const int sms = sm_count();
     if (sms <= 0)
     {
         return B200AMP_ERR_CUDA;
     }
-    auto fill = [&](int cluster) {
+    auto fill = [&](int cluster, int threads) {
         plan->cluster = cluster;
+        plan->threads = threads;
         plan->segment = static_cast<int>(((static_cast<long long>(cols) + cluster - 1) / cluster + 63) / 64 * 64);
-        plan->smem = ((plan->segment * size + 31) & ~15) + ((more + 15) & ~15) + plan->segment / 8;
+        plan->smem = ((plan->segment * size + 31) & ~15) + more(cluster, threads / 32);
     };
-    plan->threads = 256;
-    int cluster = 1;
     if (static_cast<long long>(cols) * size > MAX_CLUSTER * static_cast<long long>(MAX_ROW_SMEM))
     {
-        set_error("rows of %d columns are beyond the maximum of %lld", cols, MAX_CLUSTER * static_cast<long long>(MAX_ROW_SMEM) / size);
+        set_error("rows of %d columns are beyond the maximum of %lld", cols,
+                  MAX_CLUSTER * static_cast<long long>(MAX_ROW_SMEM) / size);
         return B200AMP_ERR_LIMIT;
     }
-    for (fill(1); cluster < MAX_CLUSTER && plan->smem > 55 * 1024; fill(cluster))
+    int cluster = 1;
+    for (fill(1, 256); cluster < MAX_CLUSTER && plan->smem > 56 * 1024; fill(cluster, 256))
     {
         cluster *= 2;
     }
     while (cluster < MAX_CLUSTER && rows * cluster < sms && plan->segment > 2048)
     {
         cluster *= 2;
-        fill(cluster);
+        fill(cluster, 256);
     }
     if (plan->segment * size <= 12 * 1024)
     {
-        plan->threads = 128;
+        fill(cluster, 128);
     }
     if (plan->smem > MAX_ROW_SMEM)
     {
@@ -260,7 +262,7 @@ struct RowTile
 
 // Blocks of a kernel that fit the device at once, as whole clusters (asked once for each shape).
 template <typename Kernel>
-int resident_clusters(Kernel kernel, const RowPlan &plan, int *clusters)
+int resident_clusters(Kernel kernel, const RowPlan &plan, int threads, int *clusters)
 {
     struct Known
     {
@@ -285,7 +287,7 @@ int resident_clusters(Kernel kernel, const RowPlan &plan, int *clusters)
     B200AMP_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(plan.cluster);
-    config.blockDim = dim3(plan.threads);
+    config.blockDim = dim3(threads);
     config.dynamicSmemBytes = plan.smem;
     cudaLaunchAttribute attribute[1];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -306,10 +308,10 @@ int resident_clusters(Kernel kernel, const RowPlan &plan, int *clusters)
 }
 
 template <typename Kernel, typename Args>
-int launch_rows(Kernel kernel, const Args &args, RowPlan plan, long long rows, cudaStream_t stream)
+int launch_rows(Kernel kernel, const Args &args, RowPlan plan, int threads, long long rows, cudaStream_t stream)
 {
     int clusters = 0;
-    const int rc = resident_clusters(kernel, plan, &clusters);
+    const int rc = resident_clusters(kernel, plan, threads, &clusters);
     if (rc != B200AMP_OK)
     {
         return rc;
@@ -317,7 +319,7 @@ int launch_rows(Kernel kernel, const Args &args, RowPlan plan, long long rows, c
     clusters = static_cast<int>(rows < 1 ? 1 : rows < clusters ? rows : clusters);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(clusters * plan.cluster);
-    config.blockDim = dim3(plan.threads);
+    config.blockDim = dim3(threads);
     config.dynamicSmemBytes = plan.smem;
     config.stream = stream;
     cudaLaunchAttribute attribute[1];

@@ -17,6 +17,9 @@
 namespace b200amp
 {
 
+// Set when a wait for a row's copy ran out. Read by b200amp_device_error().
+__device__ int g_row_timeout = 0;
+
 struct DistillArgs
 {
     const void *logits;
@@ -88,14 +91,29 @@ __host__ __device__ inline int row_sums_bytes(int blocks, int n_warps)
     return blocks * static_cast<int>(4 * sizeof(double) + 2 * sizeof(float)) + n_warps * static_cast<int>(3 * sizeof(float));
 }
 
+// fp64 functions as calls: inlined a dozen times, code that a single warp runs through once a row is fetched more
+// slowly than it is executed.
+__device__ __noinline__ double exp64(double x)
+{
+    return exp(x);
+}
+
 // e^((from - to) f), 0 from -inf
 __device__ __forceinline__ double shifted(float from, float to, double f)
 {
-    return from == -INFINITY ? 0.0 : from == to ? 1.0 : exp((static_cast<double>(from) - static_cast<double>(to)) * f);
+    return from == -INFINITY ? 0.0 : exp64((static_cast<double>(from) - static_cast<double>(to)) * f);
 }
 __device__ __forceinline__ float shifted_fast(float from, float to, float c)
 {
     return from == -INFINITY ? 0.0f : exp2_fast((from - to) * c);
+}
+
+// Maximum over the warp with NaN winning, in one instruction.
+__device__ __forceinline__ float warp_max_once(float v)
+{
+    float m;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
 }
 
 // Sum over the first n lanes (a power of two), in every lane.
@@ -212,6 +230,7 @@ __device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, 
     {
         reinterpret_cast<Vec16<T> *>(tile.buf)[i] = gradient_of<TWO>(tile, i, ref, c_t, c_1, f_t, f_1);
     }
+    before_copies();
     sweep_barrier<THREADS>();
     for (int i = tid; i < tile.held; i += THREADS)
     {
@@ -220,11 +239,12 @@ __device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, 
 }
 
 // A cluster a row, the row in its shared memory between the sweeps. A block has SWEEP threads that sweep the segment
-// and one more warp for what there is one of a row: the record, the factors, the loss, the listed columns. That warp
-// works while the others sweep, so its fp64 chains are off the row's path, and they are issued once a block and not once
-// a warp (done by every warp they were two thirds of all instructions). Barriers of a block and row:
-//     arrived   the row is in shared memory
-//     marked    the listed columns and the label have been taken out of it
+// and one more warp for what there is one of a row: the listed columns' sums, the factors, the loss. That warp works
+// while the others sweep, so its fp64 chains are off the row's path, and they are issued once a block and not once a
+// warp (done by every warp they were two thirds of all instructions). The sweeping threads read the record while the
+// row is on its way. Barriers of a block and row:
+//     arrived   the row is in shared memory, the record has been read
+//     marked    the listed columns and the label have been taken out of the row
 //     summed    (the cluster's) every warp's sums are with every block
 //     factors   the row's factors are known
 //     written   the gradient is out; the row's place may be filled again
@@ -236,7 +256,9 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
     constexpr int THREADS = SWEEP + 32, WARPS = SWEEP / 32;     // WARPS: those that sweep
     extern __shared__ __align__(16) char dynamic[];
     __shared__ double scratch[THREADS / 32];
-    __shared__ float shared_ref, shared_f_t, shared_f_1;
+    __shared__ float shared_ref, shared_f_t, shared_f_1, t_max_of[WARPS];
+    __shared__ int label_listed[2], beyond_listed[2];
+    __shared__ uint64_t row_bar;
     __shared__ int last_block;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool sweeps = warp < WARPS;
@@ -245,8 +267,8 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
     const int n_warps = blocks * WARPS;
     const float inf = INFINITY;
 
-    // dynamic shared memory: the segment; two rows' sums; two rows' listed columns of the segment (mass, its logarithm,
-    // logit, column); a table that finds columns listed twice
+    // dynamic shared memory: the segment; two rows' sums; two rows' records (mass, its logarithm, logit, column, -1 where
+    // that is not of this segment); a table that finds columns listed twice
     const size_t tile_bytes = (static_cast<size_t>(plan.segment) * sizeof(T) + 31) & ~static_cast<size_t>(15);
     const int sums_bytes = (row_sums_bytes(blocks, n_warps) + 7) & ~7;
     Tile tile;
@@ -256,7 +278,8 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
     double *const rec_lw0 = rec_w0 + 2 * a.k;
     float *const rec_z0 = reinterpret_cast<float *>(rec_lw0 + 2 * a.k);
     int *const rec_col0 = reinterpret_cast<int *>(rec_z0 + 2 * a.k);
-    int *const table = rec_col0 + 2 * a.k;
+    int *const mine = rec_col0 + 2 * a.k;       // places of the listed columns of this segment, in the record's order
+    int *const table = mine + a.k;
     const int table_mask = distill_table(a.k) - 1;
 
     const bool hard = a.hard != 0.0;
@@ -268,79 +291,64 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
     const int valid = max(0, min(plan.segment, a.vocab - first)), held = max(0, min(plan.segment, a.cols - first));
     const long long clusters = gridDim.x / blocks;
     auto label_of = [&](long long row) { return row >= a.rows ? -1 : a.targets != nullptr ? __ldg(&a.targets[row]) : 0; };
-    auto start = [&](long long row) {
-        if (sweeps)
+
+    // what a sweeping thread fetches of the next row's record while the gradient is swept
+    int ahead_v = -1;
+    float ahead_t = 0.0f, ahead_lse = 0.0f;
+    auto fetch = [&](long long at) {
+        if (tid < a.k)
         {
-            tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.cols);
+            ahead_v = __ldg(&a.indices[at * a.k + tid]);
+            ahead_t = load_typed(a.values, a.value_dtype, at * a.k + tid);
         }
-    };
-
-    long long row = blockIdx.x / blocks;
-    int y = label_of(row);
-    bool started = y >= 0;
-    if (started)
-    {
-        start(row);
-    }
-    const long long n_valid = count_rows<THREADS>(a.targets, a.rows, scratch);
-    const double grad_scale = static_cast<double>(a.st->loss_scale) / static_cast<double>(n_valid > 0 ? n_valid : 1);
-    const float soft_scale = a.k > 0 ? static_cast<float>(grad_scale * a.soft * inv_t) : 0.0f;
-    const float hard_scale = hard ? static_cast<float>(grad_scale * a.hard) : 0.0f;
-    for (int i = tid; i <= table_mask; i += THREADS)
-    {
-        table[i] = -1;
-    }
-    __syncthreads();
-
-    // the record of a row into rec[parity], by the last warp: its columns in this segment, in the record's order. Masses
-    // are w = e^(t / T - lse), or, before the norm that the cluster works out, e^((t - max) / T).
-    struct Record
-    {
-        int n;                  // listed columns of this segment
-        bool label_listed;      // anywhere in the row
-        double own;             // sum of their masses; NaN if a column is beyond the vocabulary
-    };
-    auto read_record = [&](long long at, int label, int parity) {
-        Record r = {0, false, 0.0};
-        double *w_of = rec_w0 + parity * a.k, *lw_of = rec_lw0 + parity * a.k;
-        float *z_of = rec_z0 + parity * a.k;
-        int *col_of = rec_col0 + parity * a.k;
-        const long long base = at * a.k;
-        double shift = 0.0;
         if (a.lse != nullptr)
         {
-            shift = __ldg(&a.lse[at]);
+            ahead_lse = __ldg(&a.lse[at]);
         }
-        else
+    };
+    // The record of a row into rec[parity], by the sweeping threads. Masses are w = e^(t / T - lse), or, before the norm
+    // that the cluster works out, e^((t - max) / T). True where this thread met a column that was listed already.
+    auto read_record = [&](long long at, int label, int parity) {
+        double *w_of = rec_w0 + parity * a.k, *lw_of = rec_lw0 + parity * a.k;
+        int *col_of = rec_col0 + parity * a.k;
+        double shift = ahead_lse;
+        if (a.lse == nullptr)
         {
-            float t_max = -inf;
-            for (int j = lane; j < a.k; j += 32)
+            float t_max = tid < a.k && ahead_v >= 0 ? ahead_t : -inf;
+            for (int j = tid + SWEEP; j < a.k; j += SWEEP)
             {
-                if (__ldg(&a.indices[base + j]) >= 0)
-                {
-                    t_max = max_nan(t_max, load_typed(a.values, a.value_dtype, base + j));
-                }
+                const float t = load_typed(a.values, a.value_dtype, at * a.k + j);
+                t_max = max_nan(t_max, __ldg(&a.indices[at * a.k + j]) >= 0 ? t : -inf);
             }
-            t_max = warp_max_nan(t_max);
+            t_max = warp_max_once(t_max);
+            if (lane == 0)
+            {
+                t_max_of[warp] = t_max;
+            }
+            sweep_barrier<SWEEP>();
+            t_max = warp_max_once(t_max_of[lane & (WARPS - 1)]);
             shift = t_max == -inf ? 0.0 : t_max * inv_t;
         }
-        bool beyond = false, twice = false;
-        for (int j0 = 0; j0 < a.k; j0 += 32)
+        bool twice = false;
+        for (int j = tid; j < a.k; j += SWEEP)
         {
-            const int j = j0 + lane;
-            const int v = j < a.k ? __ldg(&a.indices[base + j]) : -1;
-            beyond = beyond || v >= a.vocab;
-            r.label_listed = r.label_listed || (hard && v == label);
-            const bool mine = v >= first && v < first + valid;
-            const unsigned int ballot = __ballot_sync(0xffffffffu, mine);
-            if (mine)
+            const int v = j < SWEEP ? ahead_v : __ldg(&a.indices[at * a.k + j]);
+            const float t = j < SWEEP ? ahead_t : load_typed(a.values, a.value_dtype, at * a.k + j);
+            const bool of_segment = v >= first && v < first + valid;
+            col_of[j] = of_segment ? v : -1;
+            if (v >= a.vocab)
             {
-                const int to = r.n + __popc(ballot & ((1u << lane) - 1u));
-                const double lw = load_typed(a.values, a.value_dtype, base + j) * inv_t - shift, w = exp(lw);
-                lw_of[to] = lw;
-                w_of[to] = w;
-                col_of[to] = v;
-                r.own += w;
+                beyond_listed[parity] = 1;
+            }
+            if (hard && v == label)
+            {
+                label_listed[parity] = 1;
+            }
+            if (of_segment)
+            {
+                const double lw = t * inv_t - shift;
+                lw_of[j] = lw;
+                w_of[j] = exp64(lw);
                 for (int p = v & table_mask;; p = (p + 1) & table_mask)        // twice as many places as columns
                 {
                     const int there = atomicCAS(&table[p], -1, v);
@@ -351,60 +359,343 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
                     }
                 }
             }
-            r.n += __popc(ballot);
         }
-        r.label_listed = __any_sync(0xffffffffu, r.label_listed);
-        __syncwarp();
-        for (int i = lane; i <= table_mask; i += 32)
-        {
-            table[i] = -1;
-        }
-        if (__any_sync(0xffffffffu, twice))
-        {
-            // a column listed more than once keeps its first place, with all its mass
-            for (int i = lane; i < r.n; i += 32)
-            {
-                bool is_first = true;
-                double w = 0.0;
-                for (int q = 0; q < r.n; q++)
-                {
-                    is_first = is_first && !(q < i && col_of[q] == col_of[i]);
-                    w += col_of[q] == col_of[i] ? w_of[q] : 0.0;
-                }
-                z_of[i] = is_first ? 1.0f : 0.0f;
-                lw_of[i] = log(w);
-            }
-            __syncwarp();
-            for (int i = lane; i < r.n; i += 32)
-            {
-                w_of[i] = exp(lw_of[i]);
-                col_of[i] = z_of[i] != 0.0f ? col_of[i] : -1;
-            }
-        }
-        __syncwarp();
-        r.own = warp_sum_f64(r.own);
-        if (__any_sync(0xffffffffu, beyond))
-        {
-            r.own = nan("");
-        }
-        return r;
+        return twice;
     };
 
-    Record record = {0, false, 0.0};
-    if (!sweeps && y >= 0)
+    for (int i = tid; i <= table_mask; i += THREADS)
     {
-        record = read_record(row, y, 0);
+        table[i] = -1;
     }
+    if (tid < 2)
+    {
+        label_listed[tid] = 0;
+        beyond_listed[tid] = 0;
+    }
+    if (tid == 0)
+    {
+        row_barrier_init(&row_bar);
+    }
+    __syncthreads();
     if (blocks > 1)
     {
         cluster.sync();                         // every block of the cluster runs before one writes to another
     }
 
-    for (int parity = 0; row < a.rows; row += clusters)
+    // The first trip has no row yet (row < 0): it starts the first copy and reads the first record.
+    bool twice = false;
+    unsigned int loads = 0;                     // rows that have arrived
+    float soft_scale = 0.0f, hard_scale = 0.0f;
+    long long n_valid = 0;
+    int y = -1, parity = 0;
+    for (long long row = blockIdx.x / blocks - clusters; row < a.rows; row += clusters, parity ^= 1)
     {
-        T *out = a.dlogits != nullptr ? static_cast<T *>(a.dlogits) + row * a.dld : nullptr;
+        T *out = a.dlogits != nullptr && row >= 0 ? static_cast<T *>(a.dlogits) + row * a.dld : nullptr;
         const int next_y = label_of(row + clusters);
-        if (y < 0)
+        const bool label_in = hard && y >= 0 && y < a.vocab;
+        bool listed_y = false;
+        int n_listed = 0;
+        char *const place = sums + parity * sums_bytes;
+        double *const rec_w = rec_w0 + parity * a.k, *const rec_lw = rec_lw0 + parity * a.k;
+        float *const rec_z = rec_z0 + parity * a.k;
+        int *const rec_col = rec_col0 + parity * a.k;
+        float m = 0.0f, per_o = 0.0f, y_in_o = 0.0f, not_y_1 = 0.0f, total_1 = 1.0f, norm = 1.0f, poison = 0.0f;
+        float l_t = 0.0f, l_1 = 0.0f;           // the last warp's, for what it writes at the end
+        if (y >= 0)
+        {
+            if (sweeps)
+            {
+                if (!row_wait(&row_bar, loads & 1))
+                {
+                    beyond_listed[parity] = 1;  // the row is NaN
+                    g_row_timeout = 1;
+                }
+                loads++;
+            }
+            if (__syncthreads_or(twice))        // arrived
+            {
+                // a column listed more than once keeps its first place, with all its mass
+                for (int j = tid; j < a.k; j += THREADS)
+                {
+                    bool is_first = rec_col[j] >= 0;
+                    double w = 0.0;
+                    for (int q = 0; rec_col[j] >= 0 && q < a.k; q++)
+                    {
+                        is_first = is_first && !(q < j && rec_col[q] == rec_col[j]);
+                        w += rec_col[q] == rec_col[j] ? rec_w[q] : 0.0;
+                    }
+                    rec_z[j] = is_first ? 1.0f : 0.0f;
+                    rec_lw[j] = log(w);
+                }
+                __syncthreads();
+                for (int j = tid; j < a.k; j += THREADS)
+                {
+                    rec_w[j] = exp64(rec_lw[j]);
+                    rec_col[j] = rec_z[j] != 0.0f ? rec_col[j] : -1;
+                }
+                __syncthreads();
+            }
+            listed_y = label_listed[parity] != 0;
+
+            float z_y = -inf;
+            if (sweeps)
+            {
+                for (int j = tid; j < a.k; j += SWEEP)
+                {
+                    const int v = rec_col[j];
+                    if (v >= 0)
+                    {
+                        rec_z[j] = to_float(*tile.at(v));
+                        *tile.at(v) = minus_infinity<T>();
+                        before_copies();
+                    }
+                }
+            }
+            else
+            {
+                if (lane == 0 && label_in && !listed_y && y >= first && y < first + valid)
+                {
+                    // where the tile keeps column y
+                    const uintptr_t src = reinterpret_cast<uintptr_t>(static_cast<const T *>(a.logits) + row * a.ld + first);
+                    T *const e = reinterpret_cast<T *>(dynamic + (src & 15)) + (y - first);
+                    z_y = to_float(*e);
+                    *e = minus_infinity<T>();
+                    before_copies();
+                }
+                for (int j0 = 0; j0 < a.k; j0 += 32)
+                {
+                    const bool has = j0 + lane < a.k && rec_col[j0 + lane] >= 0;
+                    const unsigned int ballot = __ballot_sync(0xffffffffu, has);
+                    if (has)
+                    {
+                        mine[n_listed + __popc(ballot & ((1u << lane) - 1u))] = j0 + lane;
+                    }
+                    n_listed += __popc(ballot);
+                }
+                for (int i = lane; i <= table_mask; i += 32)
+                {
+                    table[i] = -1;
+                }
+            }
+            __syncthreads();                    // marked
+
+            if (sweeps)
+            {
+                // sums of this warp's share, relative to its own maximum
+                Vec16<T> best;
+                const T low = minus_infinity<T>();
+                T *e = reinterpret_cast<T *>(&best);
+#pragma unroll
+                for (int i = 0; i < Vec16<T>::N; i++)
+                {
+                    e[i] = low;
+                }
+                for (int i = tid; i < tile.vecs; i += SWEEP)
+                {
+                    max_into(best, tile.vec(i));
+                }
+                const float m_u = warp_max_once(max_of(best));
+                const float ref = m_u == -inf ? 0.0f : m_u;     // nothing but -inf: every term is 0
+                float s_t, s_1;
+                if (two)
+                {
+                    sweep_sums<true>(tile, ref, c_t, c_1, &s_t, &s_1);
+                }
+                else
+                {
+                    sweep_sums<false>(tile, ref, c_t, c_1, &s_t, &s_1);
+                }
+                if (lane < blocks)
+                {
+                    const RowSums to(blocks > 1 ? cluster.map_shared_rank(place, lane) : place, blocks, n_warps);
+                    to.m_u[rank * WARPS + warp] = m_u;
+                    to.s_t[rank * WARPS + warp] = s_t;
+                    to.s_1[rank * WARPS + warp] = s_1;
+                }
+            }
+            else
+            {
+                float m_l = -inf;
+                for (int i = lane; i < n_listed; i += 32)
+                {
+                    const float z = rec_z[mine[i]];
+                    m_l = max_nan(m_l, z);
+                    z_y = hard && rec_col[mine[i]] == y ? z : z_y;
+                }
+                m_l = warp_max_once(m_l);
+                z_y = warp_max_once(z_y);
+                const double ref_l = m_l == -inf ? 0.0 : m_l;
+                double lt = 0.0, l1 = 0.0, part = 0.0, own = 0.0;
+                for (int i = lane; i < n_listed; i += 32)
+                {
+                    const double d = rec_z[mine[i]] - ref_l, w = rec_w[mine[i]];
+                    lt += exp64(d * inv_t);
+                    l1 += two ? exp64(d) : 0.0;
+                    part += w != 0.0 ? w * (rec_lw[mine[i]] - d * inv_t) : 0.0;
+                    own += w;
+                }
+                if (n_listed > 0)
+                {
+                    lt = warp_sum_f64(lt);
+                    l1 = two ? warp_sum_f64(l1) : lt;
+                    part = warp_sum_f64(part);
+                    own = warp_sum_f64(own);
+                }
+                if (beyond_listed[parity] != 0)
+                {
+                    own = nan("");              // a column beyond the vocabulary: the row is NaN
+                }
+                if (lane < blocks)
+                {
+                    const RowSums to(blocks > 1 ? cluster.map_shared_rank(place, lane) : place, blocks, n_warps);
+                    to.l_t[rank] = lt;
+                    to.l_1[rank] = l1;
+                    to.part[rank] = part;
+                    to.own[rank] = own;
+                    to.m_l[rank] = m_l;
+                    to.z_y[rank] = z_y;
+                }
+            }
+            if (blocks > 1)
+            {
+                cluster.sync();                 // summed
+            }
+            else
+            {
+                __syncthreads();
+            }
+
+            if (sweeps)
+            {
+                if (next_y >= 0)
+                {
+                    fetch(row + clusters);
+                }
+                both_barrier<THREADS>();        // factors
+                if (out != nullptr && tile.vecs > 0)
+                {
+                    if (two)
+                    {
+                        sweep_gradient<true>(tile, out, shared_ref, c_t, c_1, shared_f_t, shared_f_1);
+                    }
+                    else
+                    {
+                        sweep_gradient<false>(tile, out, shared_ref, c_t, c_1, shared_f_t, shared_f_1);
+                    }
+                }
+            }
+            else
+            {
+                // the row's factors; fp32 does for the gradient
+                const RowSums all(place, blocks, n_warps);
+                const bool is_block = lane < blocks;
+                const float block_l = is_block ? all.m_l[lane] : -inf;
+                const double block_lt = is_block ? all.l_t[lane] : 0.0, block_l1 = is_block ? all.l_1[lane] : 0.0;
+                const double block_own = is_block ? all.own[lane] : 0.0, block_part = is_block ? all.part[lane] : 0.0;
+                float all_u = -inf;
+                for (int i = lane; i < n_warps; i += 32)
+                {
+                    all_u = max_nan(all_u, all.m_u[i]);
+                }
+                all_u = warp_max_once(all_u);
+                z_y = warp_max_once(is_block ? all.z_y[lane] : -inf);
+                const float m_o = listed_y ? all_u : max_nan(all_u, z_y);       // of the columns not listed
+                m = max_nan(m_o, warp_max_once(block_l));
+                float u_t = 0.0f, u_1 = 0.0f;
+                for (int i = lane; i < n_warps; i += 32)
+                {
+                    const float in_u = shifted_fast(all.m_u[i], all_u, c_t);
+                    u_t = fmaf(all.s_t[i], in_u, u_t);
+                    u_1 += two ? all.s_1[i] * shifted_fast(all.m_u[i], all_u, c_1) : 0.0f;
+                }
+                u_t = warp_sum_f32(u_t);
+                u_1 = two ? warp_sum_f32(u_1) : u_t;
+                const float listed_t = sum_lanes(static_cast<float>(block_lt) * shifted_fast(block_l, m, c_t), blocks);
+                const float listed_1 =
+                    two ? sum_lanes(static_cast<float>(block_l1) * shifted_fast(block_l, m, c_1), blocks) : listed_t;
+                const double own = sum_lanes(block_own, blocks);
+                // mass of the listed columns; what a w is multiplied by
+                norm = a.lse != nullptr || own == 0.0 ? 1.0f : __fdividef(1.0f, static_cast<float>(own));
+                const double mass = a.lse != nullptr || own == 0.0 || own != own ? own : 1.0;
+                const float u_in_o = shifted_fast(all_u, m_o, c_t);
+                y_in_o = listed_y ? 0.0f : shifted_fast(z_y, m_o, c_t);
+                const float others = fmaf(u_t, u_in_o, y_in_o);
+                const float o_in_all = shifted_fast(m_o, m, c_t);
+                const float total = fmaf(others, o_in_all, listed_t);
+                const double rest = a.lse != nullptr && a.k > 0 && others > 0.0f ? fmax(0.0, 1.0 - mass) : 0.0;
+                poison = !isfinite(m) || (hard && !label_in) ? NAN : 0.0f;
+                const float whole = static_cast<float>(mass + rest) + poison;
+                const float u_in_all_1 = two ? shifted_fast(all_u, m, c_1) : u_in_o * o_in_all;
+                not_y_1 = fmaf(u_1, u_in_all_1, listed_1);                      // all but the label, where that is not listed
+                total_1 = not_y_1 + (listed_y ? 0.0f : shifted_fast(z_y, m, c_1));
+                const float q_per = soft_scale * __fdividef(whole, total);
+                per_o = q_per * o_in_all - (rest > 0.0 ? soft_scale * __fdividef(static_cast<float>(rest), others) : 0.0f);
+                l_1 = hard ? __fdividef(hard_scale, total_1) : 0.0f;
+                l_t = q_per + (two ? 0.0f : l_1);
+                const float f_1 = l_1 * u_in_all_1;
+                if (lane == 0)
+                {
+                    beyond_listed[parity] = 0;
+                    label_listed[parity] = 0;
+                    shared_ref = all_u == -inf ? 0.0f : all_u;
+                    shared_f_t = per_o * u_in_o + poison + (two ? 0.0f : f_1);
+                    shared_f_1 = f_1;
+                }
+                both_barrier<THREADS>();        // factors
+
+                // while the gradient is swept: the loss, in fp64, in turn by the cluster's blocks
+                if (rank == static_cast<int>(row / clusters & (blocks - 1)))
+                {
+                    double u_t64 = 0.0, u_164 = 0.0;
+                    for (int i = lane; i < n_warps; i += 32)
+                    {
+                        u_t64 += all.s_t[i] * shifted(all.m_u[i], all_u, inv_t);
+                        u_164 += two ? all.s_1[i] * shifted(all.m_u[i], all_u, 1.0) : 0.0;
+                    }
+                    u_t64 = warp_sum_f64(u_t64);
+                    u_164 = two ? warp_sum_f64(u_164) : u_t64;
+                    // the other powers, one a lane: the blocks' listed sums, then what is not listed
+                    const float from = is_block ? block_l : lane == 16 || lane == 19 ? all_u : lane == 18 ? m_o : z_y;
+                    const float to = lane == 16 || lane == 17 ? m_o : m;
+                    const double e = shifted(from, to, lane < 19 ? inv_t : 1.0);
+                    const double listed_t64 = sum_lanes(block_lt * e, blocks);
+                    const double listed_164 =
+                        two ? sum_lanes(is_block ? block_l1 * shifted(block_l, m, 1.0) : 0.0, blocks) : listed_t64;
+                    const double ref_l = block_l == -inf ? 0.0 : block_l;
+                    const double part =
+                        sum_lanes(block_part + (block_own != 0.0 ? block_own * (m - ref_l) * inv_t : 0.0), blocks);
+                    const double u_in_o64 = __shfl_sync(0xffffffffu, e, 16), y_in_o64 = __shfl_sync(0xffffffffu, e, 17);
+                    const double o_in_all64 = __shfl_sync(0xffffffffu, e, 18), u_in_all64 = __shfl_sync(0xffffffffu, e, 19);
+                    const double y_in_all64 = __shfl_sync(0xffffffffu, e, 20);
+                    const double o = u_t64 * u_in_o64 + (listed_y ? 0.0 : y_in_o64);
+                    const double s = o * o_in_all64 + listed_t64;
+                    const double s_1 = u_164 * (two ? u_in_all64 : u_in_o64 * o_in_all64) + listed_164 + (listed_y ? 0.0 : y_in_all64);
+                    // one logarithm a lane
+                    const double of = lane == 0 ? s : lane == 1 ? s_1 : lane == 2 ? o : lane == 3 ? rest : own;
+                    const double log_of = of > 0.0 ? log(of) : 0.0;
+                    const double log_s = __shfl_sync(0xffffffffu, log_of, 0), log_s1 = __shfl_sync(0xffffffffu, log_of, 1);
+                    const double log_o = __shfl_sync(0xffffffffu, log_of, 2), log_rest = __shfl_sync(0xffffffffu, log_of, 3);
+                    const double log_own = __shfl_sync(0xffffffffu, log_of, 4);
+                    if (lane == 0)
+                    {
+                        double loss = 0.0;
+                        if (a.k > 0)
+                        {
+                            loss = a.lse != nullptr ? part : own == 0.0 ? 0.0 : part / own - log_own;
+                            loss += (mass + rest) * log_s;
+                            loss += rest > 0.0 ? rest * (log_rest - log_o - (static_cast<double>(m_o) - m) * inv_t) : 0.0;
+                            loss *= a.soft;
+                        }
+                        if (hard)
+                        {
+                            loss += a.hard * (log_s1 - (static_cast<double>(z_y) - m));
+                        }
+                        a.row_loss[row] = static_cast<float>(loss + poison);
+                    }
+                }
+            }
+        }
+        else if (row >= 0)
         {
             for (int i = tid; out != nullptr && i < held; i += THREADS)
             {
@@ -414,284 +705,52 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
             {
                 a.row_loss[row] = 0.0f;
             }
-            if (!sweeps && next_y >= 0)
-            {
-                record = read_record(row + clusters, next_y, parity);
-            }
-            y = next_y;
-            started = false;
-            continue;
         }
-        if (!started)
-        {
-            start(row);
-        }
-        const bool label_in = hard && y < a.vocab;
-        char *const place = sums + parity * sums_bytes;
-        double *const rec_w = rec_w0 + parity * a.k, *const rec_lw = rec_lw0 + parity * a.k;
-        float *const rec_z = rec_z0 + parity * a.k;
-        int *const rec_col = rec_col0 + parity * a.k;
-        if (sweeps)
-        {
-            copy_async_wait();
-        }
-        __syncthreads();                        // arrived
 
-        float m_l = -inf, z_y = -inf;
-        if (!sweeps)
+        if (y >= 0)
         {
-            // where column v of this segment is: the tile's own reckoning, which the sweeping threads hold
-            const uintptr_t src = reinterpret_cast<uintptr_t>(static_cast<const T *>(a.logits) + row * a.ld + first);
-            T *const e = reinterpret_cast<T *>(dynamic + (src & 15)) - first;
-            for (int i = lane; i < record.n; i += 32)
+            both_barrier<THREADS>();            // written
+        }
+        twice = false;
+        if (sweeps && next_y >= 0)
+        {
+            tile.start(static_cast<const T *>(a.logits) + (row + clusters) * a.ld, first, plan.segment, a.vocab, a.cols,
+                       &row_bar);
+            if (a.k > 0)
             {
-                const int v = rec_col[i];
-                if (v >= 0)
+                if (y < 0)
                 {
-                    const float z = to_float(e[v]);
-                    e[v] = minus_infinity<T>();
-                    rec_z[i] = z;
-                    m_l = max_nan(m_l, z);
-                    z_y = hard && v == y ? z : z_y;
+                    fetch(row + clusters);
                 }
-            }
-            if (lane == 0 && label_in && !record.label_listed && y >= first && y < first + valid)
-            {
-                z_y = to_float(e[y]);
-                e[y] = minus_infinity<T>();
+                twice = read_record(row + clusters, next_y, parity ^ 1);
             }
         }
-        __syncthreads();                        // marked
-
-        if (sweeps)
+        if (row < 0)
         {
-            // sums of this warp's share, relative to its own maximum
-            Vec16<T> best;
-            const T low = minus_infinity<T>();
-            T *e = reinterpret_cast<T *>(&best);
-#pragma unroll
-            for (int i = 0; i < Vec16<T>::N; i++)
-            {
-                e[i] = low;
-            }
-            for (int i = tid; i < tile.vecs; i += SWEEP)
-            {
-                max_into(best, tile.vec(i));
-            }
-            const float m_u = warp_max_nan(max_of(best));
-            const float ref = m_u == -inf ? 0.0f : m_u;         // nothing but -inf: every term is 0
-            float s_t, s_1;
-            if (two)
-            {
-                sweep_sums<true>(tile, ref, c_t, c_1, &s_t, &s_1);
-            }
-            else
-            {
-                sweep_sums<false>(tile, ref, c_t, c_1, &s_t, &s_1);
-            }
-            if (lane < blocks)
-            {
-                const RowSums to(blocks > 1 ? cluster.map_shared_rank(place, lane) : place, blocks, n_warps);
-                to.m_u[rank * WARPS + warp] = m_u;
-                to.s_t[rank * WARPS + warp] = s_t;
-                to.s_1[rank * WARPS + warp] = s_1;
-            }
+            n_valid = count_rows<THREADS>(a.targets, a.rows, scratch);
+            const double scale = static_cast<double>(a.st->loss_scale) / static_cast<double>(n_valid > 0 ? n_valid : 1);
+            soft_scale = a.k > 0 ? static_cast<float>(scale * a.soft * inv_t) : 0.0f;
+            hard_scale = hard ? static_cast<float>(scale * a.hard) : 0.0f;
         }
-        else
+        if (!sweeps && y >= 0 && out != nullptr)
         {
-            m_l = warp_max_nan(m_l);
-            z_y = warp_max_nan(z_y);
-            const double ref_l = m_l == -inf ? 0.0 : m_l;
-            double l_t = 0.0, l_1 = 0.0, part = 0.0;
-            for (int i = lane; i < record.n; i += 32)
+            // while the next row is on its way: what the sweep left to this warp
+            const float p_scale = soft_scale * norm;
+            for (int i = lane; i < n_listed; i += 32)
             {
-                if (rec_col[i] >= 0)
-                {
-                    const double d = rec_z[i] - ref_l, w = rec_w[i];
-                    l_t += exp(d * inv_t);
-                    l_1 += two ? exp(d) : 0.0;
-                    part += w != 0.0 ? w * (rec_lw[i] - d * inv_t) : 0.0;
-                }
-            }
-            if (record.n > 0)
-            {
-                l_t = warp_sum_f64(l_t);
-                l_1 = two ? warp_sum_f64(l_1) : l_t;
-                part = warp_sum_f64(part);
-            }
-            if (lane < blocks)
-            {
-                const RowSums to(blocks > 1 ? cluster.map_shared_rank(place, lane) : place, blocks, n_warps);
-                to.l_t[rank] = l_t;
-                to.l_1[rank] = l_1;
-                to.part[rank] = part;
-                to.own[rank] = record.own;
-                to.m_l[rank] = m_l;
-                to.z_y[rank] = z_y;
-            }
-        }
-        if (blocks > 1)
-        {
-            cluster.sync();                     // summed
-        }
-        else
-        {
-            __syncthreads();
-        }
-
-        if (sweeps)
-        {
-            both_barrier<THREADS>();            // factors
-            if (out != nullptr && tile.vecs > 0)
-            {
+                const int j = mine[i], v = rec_col[j];
+                float g = fmaf(shifted_fast(rec_z[j], m, c_t), l_t, -p_scale * static_cast<float>(rec_w[j])) + poison;
                 if (two)
                 {
-                    sweep_gradient<true>(tile, out, shared_ref, c_t, c_1, shared_f_t, shared_f_1);
+                    g = fmaf(shifted_fast(rec_z[j], m, c_1), l_1, g);
                 }
-                else
-                {
-                    sweep_gradient<false>(tile, out, shared_ref, c_t, c_1, shared_f_t, shared_f_1);
-                }
+                out[v] = from_float<T>(hard && v == y ? g - hard_scale : g);
             }
-            both_barrier<THREADS>();            // written
-            started = next_y >= 0;
-            if (started)
+            if (lane == 0 && label_in && !listed_y && y >= first && y < first + valid)
             {
-                start(row + clusters);
+                out[y] = from_float<T>(per_o * y_in_o - hard_scale * __fdividef(not_y_1, total_1) + poison);
             }
         }
-        else
-        {
-            // the row's factors; fp32 does for the gradient
-            const RowSums all(place, blocks, n_warps);
-            const bool listed_y = record.label_listed;
-            float all_u = -inf;
-            for (int i = lane; i < n_warps; i += 32)
-            {
-                all_u = max_nan(all_u, all.m_u[i]);
-            }
-            const bool is_block = lane < blocks;
-            const float block_l = is_block ? all.m_l[lane] : -inf;
-            const double block_lt = is_block ? all.l_t[lane] : 0.0, block_l1 = is_block ? all.l_1[lane] : 0.0;
-            const double block_own = is_block ? all.own[lane] : 0.0, block_part = is_block ? all.part[lane] : 0.0;
-            all_u = warp_max_nan(all_u);
-            float all_l = block_l;
-            z_y = is_block ? all.z_y[lane] : -inf;
-            for (int offset = blocks >> 1; offset > 0; offset >>= 1)
-            {
-                all_l = max_nan(all_l, __shfl_xor_sync(0xffffffffu, all_l, offset));
-                z_y = max_nan(z_y, __shfl_xor_sync(0xffffffffu, z_y, offset));
-            }
-            all_l = __shfl_sync(0xffffffffu, all_l, 0);
-            z_y = __shfl_sync(0xffffffffu, z_y, 0);
-            const float m_o = listed_y ? all_u : max_nan(all_u, z_y);       // of the columns not listed
-            const float m = max_nan(m_o, all_l);
-            float u_t = 0.0f, u_1 = 0.0f;
-            for (int i = lane; i < n_warps; i += 32)
-            {
-                const float in_u = shifted_fast(all.m_u[i], all_u, c_t);
-                u_t = fmaf(all.s_t[i], in_u, u_t);
-                u_1 += two ? all.s_1[i] * shifted_fast(all.m_u[i], all_u, c_1) : 0.0f;
-            }
-            u_t = warp_sum_f32(u_t);
-            u_1 = two ? warp_sum_f32(u_1) : u_t;
-            const float listed_t = sum_lanes(static_cast<float>(block_lt) * shifted_fast(block_l, m, c_t), blocks);
-            const float listed_1 = two ? sum_lanes(static_cast<float>(block_l1) * shifted_fast(block_l, m, c_1), blocks) : listed_t;
-            const double own = sum_lanes(block_own, blocks);
-            // mass of the listed columns, and what a w is multiplied by
-            const double mass = a.lse != nullptr ? own : own == 0.0 ? 0.0 : own / own;
-            const double norm = a.lse != nullptr || own == 0.0 ? 1.0 : 1.0 / own;
-            const float u_in_o = shifted_fast(all_u, m_o, c_t), y_in_o = listed_y ? 0.0f : shifted_fast(z_y, m_o, c_t);
-            const float others = fmaf(u_t, u_in_o, y_in_o);
-            const float o_in_all = shifted_fast(m_o, m, c_t);
-            const float total = fmaf(others, o_in_all, listed_t);
-            const double rest = a.lse != nullptr && a.k > 0 && others > 0.0f ? fmax(0.0, 1.0 - mass) : 0.0;
-            const float poison = !isfinite(m) || (hard && !label_in) ? NAN : 0.0f;
-            const float whole = static_cast<float>(mass + rest) + poison;
-            const float u_in_all_1 = two ? shifted_fast(all_u, m, c_1) : u_in_o * o_in_all;
-            const float not_y_1 = fmaf(u_1, u_in_all_1, listed_1);          // all but the label, where that is not listed
-            const float total_1 = not_y_1 + (listed_y ? 0.0f : shifted_fast(z_y, m, c_1));
-            const float per_o = whole * o_in_all / total - (rest > 0.0 ? static_cast<float>(rest) / others : 0.0f);
-            const float f_1 = hard ? hard_scale * u_in_all_1 / total_1 : 0.0f;
-            if (lane == 0)
-            {
-                shared_ref = all_u == -inf ? 0.0f : all_u;
-                shared_f_t = soft_scale * per_o * u_in_o + poison + (two ? 0.0f : f_1);
-                shared_f_1 = f_1;
-            }
-            both_barrier<THREADS>();            // factors
-
-            // while the gradient is swept: the loss, in fp64, and the next row's record
-            if (rank == 0)
-            {
-                double u_t64 = 0.0, u_164 = 0.0;
-                for (int i = lane; i < n_warps; i += 32)
-                {
-                    const double in_u = shifted(all.m_u[i], all_u, inv_t);
-                    u_t64 += all.s_t[i] * in_u;
-                    u_164 += two ? all.s_1[i] * shifted(all.m_u[i], all_u, 1.0) : 0.0;
-                }
-                u_t64 = warp_sum_f64(u_t64);
-                u_164 = two ? warp_sum_f64(u_164) : u_t64;
-                const double listed_t64 = sum_lanes(block_lt * shifted(block_l, m, inv_t), blocks);
-                const double listed_164 = two ? sum_lanes(block_l1 * shifted(block_l, m, 1.0), blocks) : listed_t64;
-                const double ref_l = block_l == -inf ? 0.0 : block_l;
-                const double part = sum_lanes(block_part + (block_own != 0.0 ? block_own * (m - ref_l) * inv_t : 0.0), blocks);
-                const double o = u_t64 * shifted(all_u, m_o, inv_t) + (listed_y ? 0.0 : shifted(z_y, m_o, inv_t));
-                const double s = o * shifted(m_o, m, inv_t) + listed_t64;
-                const double s_1 = u_164 * shifted(all_u, m, two ? 1.0 : inv_t) + listed_164 + (listed_y ? 0.0 : shifted(z_y, m, 1.0));
-                // one logarithm a lane
-                const double of = lane == 0 ? s : lane == 1 ? s_1 : lane == 2 ? o : lane == 3 ? rest : norm;
-                const double log_of = of > 0.0 ? log(of) : 0.0;
-                const double log_s = __shfl_sync(0xffffffffu, log_of, 0), log_s1 = __shfl_sync(0xffffffffu, log_of, 1);
-                const double log_o = __shfl_sync(0xffffffffu, log_of, 2), log_rest = __shfl_sync(0xffffffffu, log_of, 3);
-                const double log_norm = __shfl_sync(0xffffffffu, log_of, 4);
-                if (lane == 0)
-                {
-                    double loss = 0.0;
-                    if (a.k > 0)
-                    {
-                        loss = part * norm + mass * log_norm + (mass + rest) * log_s;
-                        loss += rest > 0.0 ? rest * (log_rest - log_o - (static_cast<double>(m_o) - m) * inv_t) : 0.0;
-                        loss *= a.soft;
-                    }
-                    if (hard)
-                    {
-                        loss += a.hard * (log_s1 - (static_cast<double>(z_y) - m));
-                    }
-                    a.row_loss[row] = static_cast<float>(loss + poison);
-                }
-            }
-            const int n_listed = record.n;
-            if (next_y >= 0)
-            {
-                record = read_record(row + clusters, next_y, parity ^ 1);
-            }
-            both_barrier<THREADS>();            // written
-
-            // while the next row is on its way: what the gradient's sweep left to this warp
-            const float l_t = soft_scale * whole / total + (hard && !two ? hard_scale / total_1 : 0.0f);
-            const float l_1 = two ? hard_scale / total_1 : 0.0f;
-            for (int i = lane; out != nullptr && i < n_listed; i += 32)
-            {
-                const int v = rec_col[i];
-                if (v >= 0)
-                {
-                    float g = fmaf(shifted_fast(rec_z[i], m, c_t), l_t, -soft_scale * static_cast<float>(rec_w[i] * norm)) + poison;
-                    if (two)
-                    {
-                        g = fmaf(shifted_fast(rec_z[i], m, c_1), l_1, g);
-                    }
-                    out[v] = from_float<T>(hard && v == y ? g - hard_scale : g);
-                }
-            }
-            if (out != nullptr && lane == 0 && label_in && !listed_y && y >= first && y < first + valid)
-            {
-                out[y] = from_float<T>(soft_scale * per_o * y_in_o - hard_scale * (not_y_1 / total_1) + poison);
-            }
-            started = next_y >= 0;
-        }
-        parity ^= 1;
         y = next_y;
     }
 
@@ -699,15 +758,15 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
     {
         return;
     }
-    double mine = 0.0;
+    double loss_sum = 0.0;
     for (long long i = tid; i < a.rows; i += THREADS)
     {
-        mine += static_cast<double>(__ldcg(&a.row_loss[i]));
+        loss_sum += static_cast<double>(__ldcg(&a.row_loss[i]));
     }
-    mine = block_sum_f64<THREADS>(mine, scratch);
+    loss_sum = block_sum_f64<THREADS>(loss_sum, scratch);
     if (tid == 0)
     {
-        a.st->loss = static_cast<float>(mine / static_cast<double>(n_valid > 0 ? n_valid : 1));
+        a.st->loss = static_cast<float>(loss_sum / static_cast<double>(n_valid > 0 ? n_valid : 1));
         a.st->n_valid = static_cast<int>(n_valid);
     }
 }
@@ -721,7 +780,7 @@ static int launch_distill(const DistillArgs &a, RowPlan plan, cudaStream_t strea
 template <typename T>
 static int launch_distill(const DistillArgs &a, cudaStream_t stream)
 {
-    const int record = 2 * a.k * (2 * sizeof(double) + sizeof(float) + sizeof(int)) + distill_table(a.k) * sizeof(int);
+    const int record = 2 * a.k * (2 * sizeof(double) + sizeof(float) + sizeof(int)) + (a.k + distill_table(a.k)) * sizeof(int);
     RowPlan plan;
     const int rc = plan_rows(
         a.rows, a.cols, sizeof(T),
@@ -731,6 +790,18 @@ static int launch_distill(const DistillArgs &a, cudaStream_t stream)
         return rc;
     }
     return plan.threads == 128 ? launch_distill<T, 128>(a, plan, stream) : launch_distill<T, 256>(a, plan, stream);
+}
+
+// *out = 1 if a wait for a row's copy gave up since the last call (clears it).
+int row_timeout_take(int *out)
+{
+    B200AMP_CUDA(cudaMemcpyFromSymbol(out, g_row_timeout, sizeof(int)));
+    if (*out != 0)
+    {
+        const int zero = 0;
+        B200AMP_CUDA(cudaMemcpyToSymbol(g_row_timeout, &zero, sizeof(int)));
+    }
+    return B200AMP_OK;
 }
 
 } // namespace b200amp

@@ -600,7 +600,8 @@ extern "C" B200AMP_API int b200amp_pass2_f16_runs(float *master, float *m, float
 
 // What gave up a bounded wait on the current device since the last call, as a bit mask (the flags
 // are cleared by reading them): 1 = a shared-memory staged launch waiting for a bulk copy,
-// 2 = a ZeRO-1 kernel waiting for another rank. Synchronises the device.
+// 2 = a ZeRO-1 kernel waiting for another rank, 4 = a loss kernel waiting for a row's copy.
+// Synchronises the device.
 extern "C" B200AMP_API int b200amp_device_error(int *out)
 {
     B200AMP_REQUIRE(out != nullptr, "device_error: out is null");
@@ -617,6 +618,12 @@ extern "C" B200AMP_API int b200amp_device_error(int *out)
     {
         return rc;
     }
-    *out = (flag != 0 ? 1 : 0) | (rank_wait != 0 ? 2 : 0);
+    int row_wait = 0;
+    rc = row_timeout_take(&row_wait);
+    if (rc != B200AMP_OK)
+    {
+        return rc;
+    }
+    *out = (flag != 0 ? 1 : 0) | (rank_wait != 0 ? 2 : 0) | (row_wait != 0 ? 4 : 0);
     return B200AMP_OK;
 }

@@ -195,16 +195,52 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
     return r;
 }
 
-__device__ __forceinline__ void copy_async16(void *dst_smem, const void *src_gmem)
+// Bulk copies: one thread hands a whole segment to the copy engine, which completes its bytes on a barrier in shared
+// memory. (Copied by cp.async, 16 bytes a thread, the threads themselves wait for the memory system to take the
+// requests: a fifth of a row's time.)
+__device__ __forceinline__ uint32_t shared_address(const void *p)
 {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;"
-                 :
-                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst_smem))), "l"(src_gmem)
-                 : "memory");
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
-__device__ __forceinline__ void copy_async_wait()
+__device__ __forceinline__ void row_barrier_init(uint64_t *bar)
 {
-    asm volatile("cp.async.wait_all;" : : : "memory");
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" : : "r"(shared_address(bar)) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" : : : "memory");
+}
+__device__ __forceinline__ void row_copy(void *dst, const void *src, unsigned bytes, uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" : : "r"(shared_address(bar)), "r"(bytes) : "memory");
+    if (bytes > 0)
+    {
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     :
+                     : "r"(shared_address(dst)), "l"(src), "r"(bytes), "r"(shared_address(bar))
+                     : "memory");
+    }
+}
+// Bounded: false when the limit ran out (about a second), which only a copy that never completes can bring about.
+__device__ __forceinline__ bool row_wait(uint64_t *bar, unsigned parity)
+{
+    for (unsigned tries = 0; tries < 1u << 22; tries++)
+    {
+        unsigned ok;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(shared_address(bar)), "r"(parity)
+                     : "memory");
+        if (ok != 0)
+        {
+            return true;
+        }
+    }
+    return false;
+}
+// What this thread wrote to shared memory comes before copies that are started after a barrier.
+__device__ __forceinline__ void before_copies()
+{
+    asm volatile("fence.proxy.async.shared::cta;" : : : "memory");
 }
 
 // This block's segment of the current row.
@@ -231,9 +267,9 @@ struct RowTile
         return reinterpret_cast<const Vec16<T> *>(buf)[i];
     }
 
-    // Starts the copy of columns [first, first + valid) of the row at z; padding and ends are set to -inf.
-    // Every thread; the row is there after copy_async_wait and a barrier.
-    __device__ __forceinline__ void start(const T *z, int first_column, int segment, int vocab, int cols)
+    // Starts the copy of columns [first, first + valid) of the row at z; padding and ends are set to -inf. Every
+    // thread, after a barrier behind the last use of the segment; the row is there after row_wait and a barrier.
+    __device__ __forceinline__ void start(const T *z, int first_column, int segment, int vocab, int cols, uint64_t *bar)
     {
         first = first_column;
         valid = max(0, min(segment, vocab - first));
@@ -244,9 +280,9 @@ struct RowTile
         vecs = held > 0 ? (lead + held + N - 1) / N : 0;
         const int whole_first = lead > 0 ? 1 : 0, whole_end = (lead + valid) / N;      // vectors inside the columns
         src -= skew;
-        for (int i = whole_first + threadIdx.x; i < whole_end; i += THREADS)
+        if (threadIdx.x == 0)
         {
-            copy_async16(buf + 16 * i, src + 16ll * i);
+            row_copy(buf + 16 * whole_first, src + 16 * whole_first, 16u * max(0, whole_end - whole_first), bar);
         }
         // the elements of the other vectors: at most N - 1 at the front, then the end and the padding
         T *e = reinterpret_cast<T *>(buf);

@@ -37,17 +37,6 @@ struct DistillArgs
     LossWorkspace *ws;
 };
 
-// Places of the table that finds columns listed twice: a power of two, at least twice the listed ones.
-__host__ __device__ inline int distill_table(int k)
-{
-    int n = 2;
-    while (n < 2 * k)
-    {
-        n *= 2;
-    }
-    return n;
-}
-
 // Rows that count: every block counts for itself, as the gradient needs the number from its first row on.
 template <int THREADS>
 __device__ __forceinline__ long long count_rows(const int *targets, long long rows, double *scratch)
@@ -127,43 +116,106 @@ __device__ __forceinline__ V sum_lanes(V v, int n)
     return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// The sweeps of the segment. TWO: two softmaxes of a row, at the temperature and at 1.
+// The sweeps of the segment. TWO: two softmaxes of a row, at the temperature and at 1. They take several vectors at a
+// time: one alone leaves a warp waiting for its own loads, powers and additions.
+template <typename T, int THREADS>
+__device__ __forceinline__ float sweep_max(const RowTile<T, THREADS> &tile)
+{
+    constexpr int AT_ONCE = 4;
+    Vec16<T> best;
+    const T low = minus_infinity<T>();
+    T *e = reinterpret_cast<T *>(&best);
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::N; i++)
+    {
+        e[i] = low;
+    }
+    int i = threadIdx.x;
+    for (; i + (AT_ONCE - 1) * THREADS < tile.vecs; i += AT_ONCE * THREADS)
+    {
+        Vec16<T> v[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+        {
+            v[u] = tile.vec(i + u * THREADS);
+        }
+        max_into(v[0], v[1]);
+        max_into(v[2], v[3]);
+        max_into(best, v[0]);
+        max_into(best, v[2]);
+    }
+    for (; i < tile.vecs; i += THREADS)
+    {
+        max_into(best, tile.vec(i));
+    }
+    return warp_max_once(max_of(best));
+}
+
 template <bool TWO, typename T, int THREADS>
 __device__ __forceinline__ void sweep_sums(const RowTile<T, THREADS> &tile, float ref, float c_t, float c_1, float *s_t, float *s_1)
 {
-    constexpr int PAIRS = Vec16<T>::N / 2;
+    constexpr int PAIRS = Vec16<T>::N / 2, AT_ONCE = TWO || sizeof(T) == 2 ? 2 : 4;
     const float2 minus_ref = make_float2(-ref, -ref), c_t2 = make_float2(c_t, c_t), c_12 = make_float2(c_1, c_1);
-    float2 sum_t = make_float2(0.0f, 0.0f), sum_1 = make_float2(0.0f, 0.0f);
-    for (int i = threadIdx.x; i < tile.vecs; i += THREADS)
+    float2 sum_t[AT_ONCE], sum_1[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; u++)
     {
-        float2 f[PAIRS];
-        unpack(tile.vec(i), f);
+        sum_t[u] = make_float2(0.0f, 0.0f);
+        sum_1[u] = make_float2(0.0f, 0.0f);
+    }
+    auto add = [&](const float2 (&f)[PAIRS], int u) {
 #pragma unroll
         for (int q = 0; q < PAIRS; q++)
         {
             const float2 d = add2(f[q], minus_ref);
             const float2 x = mul2(d, c_t2);
-            sum_t = add2(sum_t, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+            sum_t[u] = add2(sum_t[u], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
             if (TWO)
             {
                 const float2 x1 = mul2(d, c_12);
-                sum_1 = add2(sum_1, make_float2(exp2_fast(x1.x), exp2_fast(x1.y)));
+                sum_1[u] = add2(sum_1[u], make_float2(exp2_fast(x1.x), exp2_fast(x1.y)));
             }
         }
+    };
+    int i = threadIdx.x;
+    for (; i + (AT_ONCE - 1) * THREADS < tile.vecs; i += AT_ONCE * THREADS)
+    {
+        float2 f[AT_ONCE][PAIRS];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+        {
+            unpack(tile.vec(i + u * THREADS), f[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+        {
+            add(f[u], u);
+        }
     }
-    *s_t = warp_sum_f32(sum_t.x + sum_t.y);
-    *s_1 = TWO ? warp_sum_f32(sum_1.x + sum_1.y) : *s_t;
+    for (; i < tile.vecs; i += THREADS)
+    {
+        float2 f[PAIRS];
+        unpack(tile.vec(i), f);
+        add(f, 0);
+    }
+#pragma unroll
+    for (int u = 1; u < AT_ONCE; u++)
+    {
+        sum_t[0] = add2(sum_t[0], sum_t[u]);
+        sum_1[0] = add2(sum_1[0], sum_1[u]);
+    }
+    *s_t = warp_sum_f32(sum_t[0].x + sum_t[0].y);
+    *s_1 = TWO ? warp_sum_f32(sum_1[0].x + sum_1[0].y) : *s_t;
 }
 
-template <bool TWO, typename T, int THREADS>
-__device__ __forceinline__ Vec16<T> gradient_of(const RowTile<T, THREADS> &tile, int i, float ref, float c_t, float c_1,
-                                                float f_t, float f_1)
+template <bool TWO, typename T>
+__device__ __forceinline__ Vec16<T> gradient_of(const Vec16<T> &z, float ref, float c_t, float c_1, float f_t, float f_1)
 {
     constexpr int PAIRS = Vec16<T>::N / 2;
     const float2 minus_ref = make_float2(-ref, -ref), c_t2 = make_float2(c_t, c_t), c_12 = make_float2(c_1, c_1);
     const float2 f_t2 = make_float2(f_t, f_t), f_12 = make_float2(f_1, f_1);
     float2 f[PAIRS];
-    unpack(tile.vec(i), f);
+    unpack(z, f);
 #pragma unroll
     for (int q = 0; q < PAIRS; q++)
     {
@@ -205,16 +257,24 @@ __device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, 
     {
         // the row starts as far from a 16-byte boundary as the logits' row: whole vectors, then the two ends
         const int whole_first = tile.lead > 0 ? 1 : 0, whole_end = (tile.lead + tile.held) / N;
-        for (int i = whole_first + tid; i < whole_end; i += THREADS)
+        int k = whole_first + tid;
+        for (; k + THREADS < whole_end; k += 2 * THREADS)
         {
-            *reinterpret_cast<uint4 *>(dst + 16ll * i) = gradient_of<TWO>(tile, i, ref, c_t, c_1, f_t, f_1).w;
+            const Vec16<T> z0 = tile.vec(k), z1 = tile.vec(k + THREADS);
+            const Vec16<T> g0 = gradient_of<TWO>(z0, ref, c_t, c_1, f_t, f_1), g1 = gradient_of<TWO>(z1, ref, c_t, c_1, f_t, f_1);
+            *reinterpret_cast<uint4 *>(dst + 16ll * k) = g0.w;
+            *reinterpret_cast<uint4 *>(dst + 16ll * (k + THREADS)) = g1.w;
+        }
+        if (k < whole_end)
+        {
+            *reinterpret_cast<uint4 *>(dst + 16ll * k) = gradient_of<TWO>(tile.vec(k), ref, c_t, c_1, f_t, f_1).w;
         }
         const bool front = tid == 0 && tile.lead > 0;
         const bool back = tid == 1 && whole_end < tile.vecs && whole_end >= whole_first;
         if (front || back)
         {
             const int i = front ? 0 : whole_end;
-            const Vec16<T> g = gradient_of<TWO>(tile, i, ref, c_t, c_1, f_t, f_1);
+            const Vec16<T> g = gradient_of<TWO>(tile.vec(i), ref, c_t, c_1, f_t, f_1);
             const T *e = reinterpret_cast<const T *>(&g);
             for (int q = 0; q < N; q++)
             {
@@ -228,7 +288,7 @@ __device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, 
     }
     for (int i = tid; i < tile.vecs; i += THREADS)
     {
-        reinterpret_cast<Vec16<T> *>(tile.buf)[i] = gradient_of<TWO>(tile, i, ref, c_t, c_1, f_t, f_1);
+        reinterpret_cast<Vec16<T> *>(tile.buf)[i] = gradient_of<TWO>(tile.vec(i), ref, c_t, c_1, f_t, f_1);
     }
     before_copies();
     sweep_barrier<THREADS>();
@@ -249,7 +309,7 @@ __device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, 
 //     factors   the row's factors are known
 //     written   the gradient is out; the row's place may be filled again
 template <typename T, int SWEEP>
-__global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(const DistillArgs a, const RowPlan plan)
+__global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(const DistillArgs a, const RowPlan plan)
 {
     namespace cg = cooperative_groups;
     using Tile = RowTile<T, SWEEP>;
@@ -268,19 +328,19 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
     const float inf = INFINITY;
 
     // dynamic shared memory: the segment; two rows' sums; two rows' records (mass, its logarithm, logit, column, -1 where
-    // that is not of this segment); a table that finds columns listed twice
+    // that is not of this segment); a bit a column, which finds those listed twice
     const size_t tile_bytes = (static_cast<size_t>(plan.segment) * sizeof(T) + 31) & ~static_cast<size_t>(15);
     const int sums_bytes = (row_sums_bytes(blocks, n_warps) + 7) & ~7;
     Tile tile;
     tile.buf = dynamic;
+    tile.uneven = (a.ld * static_cast<long long>(sizeof(T)) & 15) != 0;
     char *const sums = dynamic + tile_bytes;
     double *const rec_w0 = reinterpret_cast<double *>(sums + 2 * sums_bytes);
     double *const rec_lw0 = rec_w0 + 2 * a.k;
     float *const rec_z0 = reinterpret_cast<float *>(rec_lw0 + 2 * a.k);
     int *const rec_col0 = reinterpret_cast<int *>(rec_z0 + 2 * a.k);
     int *const mine = rec_col0 + 2 * a.k;       // places of the listed columns of this segment, in the record's order
-    int *const table = mine + a.k;
-    const int table_mask = distill_table(a.k) - 1;
+    unsigned int *const listed_bits = reinterpret_cast<unsigned int *>(mine + a.k);
 
     const bool hard = a.hard != 0.0;
     const double inv_t = a.k > 0 ? 1.0 / a.temperature : 1.0;       // the label's softmax alone is at 1
@@ -290,7 +350,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
     const int first = rank * plan.segment;
     const int valid = max(0, min(plan.segment, a.vocab - first)), held = max(0, min(plan.segment, a.cols - first));
     const long long clusters = gridDim.x / blocks;
-    auto label_of = [&](long long row) { return row >= a.rows ? -1 : a.targets != nullptr ? __ldg(&a.targets[row]) : 0; };
+    auto label_of = [&](long long row) { return row < 0 || row >= a.rows ? -1 : a.targets != nullptr ? __ldg(&a.targets[row]) : 0; };
 
     // what a sweeping thread fetches of the next row's record while the gradient is swept
     int ahead_v = -1;
@@ -349,23 +409,16 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
                 const double lw = t * inv_t - shift;
                 lw_of[j] = lw;
                 w_of[j] = exp64(lw);
-                for (int p = v & table_mask;; p = (p + 1) & table_mask)        // twice as many places as columns
-                {
-                    const int there = atomicCAS(&table[p], -1, v);
-                    if (there == -1 || there == v)
-                    {
-                        twice = twice || there == v;
-                        break;
-                    }
-                }
+                const unsigned int bit = 1u << ((v - first) & 31);
+                twice = twice || (atomicOr(&listed_bits[(v - first) >> 5], bit) & bit) != 0;
             }
         }
         return twice;
     };
 
-    for (int i = tid; i <= table_mask; i += THREADS)
+    for (int i = tid; i < plan.segment / 32; i += THREADS)
     {
-        table[i] = -1;
+        listed_bits[i] = 0u;
     }
     if (tid < 2)
     {
@@ -384,7 +437,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
 
     // The first trip has no row yet (row < 0): it starts the first copy and reads the first record.
     bool twice = false;
-    unsigned int loads = 0;                     // rows that have arrived
+    unsigned int phase = 0;                     // of row_bar
     float soft_scale = 0.0f, hard_scale = 0.0f;
     long long n_valid = 0;
     int y = -1, parity = 0;
@@ -405,12 +458,13 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
         {
             if (sweeps)
             {
-                if (!row_wait(&row_bar, loads & 1))
+                if (!row_wait(&row_bar, phase))
                 {
                     beyond_listed[parity] = 1;  // the row is NaN
                     g_row_timeout = 1;
                 }
-                loads++;
+                phase ^= 1u;
+                tile.finish();
             }
             if (__syncthreads_or(twice))        // arrived
             {
@@ -472,9 +526,10 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
                     }
                     n_listed += __popc(ballot);
                 }
-                for (int i = lane; i <= table_mask; i += 32)
+                __syncwarp();
+                for (int i = lane; i < n_listed; i += 32)
                 {
-                    table[i] = -1;
+                    listed_bits[(rec_col[mine[i]] - first) >> 5] = 0u;
                 }
             }
             __syncthreads();                    // marked
@@ -482,19 +537,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 1024 / SWEEP) distill_rows_kernel(
             if (sweeps)
             {
                 // sums of this warp's share, relative to its own maximum
-                Vec16<T> best;
-                const T low = minus_infinity<T>();
-                T *e = reinterpret_cast<T *>(&best);
-#pragma unroll
-                for (int i = 0; i < Vec16<T>::N; i++)
-                {
-                    e[i] = low;
-                }
-                for (int i = tid; i < tile.vecs; i += SWEEP)
-                {
-                    max_into(best, tile.vec(i));
-                }
-                const float m_u = warp_max_once(max_of(best));
+                const float m_u = sweep_max(tile);
                 const float ref = m_u == -inf ? 0.0f : m_u;     // nothing but -inf: every term is 0
                 float s_t, s_1;
                 if (two)
@@ -780,11 +823,14 @@ static int launch_distill(const DistillArgs &a, RowPlan plan, cudaStream_t strea
 template <typename T>
 static int launch_distill(const DistillArgs &a, cudaStream_t stream)
 {
-    const int record = 2 * a.k * (2 * sizeof(double) + sizeof(float) + sizeof(int)) + (a.k + distill_table(a.k)) * sizeof(int);
+    const int record = a.k * (2 * (2 * sizeof(double) + sizeof(float) + sizeof(int)) + sizeof(int));
     RowPlan plan;
     const int rc = plan_rows(
         a.rows, a.cols, sizeof(T),
-        [&](int blocks, int warps) { return record + 2 * ((row_sums_bytes(blocks, blocks * warps) + 7) & ~7); }, &plan);
+        [&](const RowPlan &p) {
+            return record + 2 * ((row_sums_bytes(p.cluster, p.cluster * p.threads / 32) + 7) & ~7) + p.segment / 8;
+        },
+        &plan);
     if (rc != B200AMP_OK)
     {
         return rc;

@@ -28,8 +28,8 @@ struct RowPlan
     int smem;               // dynamic shared memory of a block
 };
 
-// Cluster and block size for rows of `cols` elements of `size` bytes, with more(blocks, sweeping warps a block)
-// bytes of shared memory besides the segment. B200AMP_ERR_LIMIT where a row does not fit the largest cluster.
+// Cluster and block size for rows of `cols` elements of `size` bytes, with more(plan) bytes of shared memory
+// besides the segment. B200AMP_ERR_LIMIT where a row does not fit the largest cluster.
 template <typename More>
 int plan_rows(long long rows, int cols, int size, More more, RowPlan *plan)
 {
@@ -42,7 +42,7 @@ int plan_rows(long long rows, int cols, int size, More more, RowPlan *plan)
         plan->cluster = cluster;
         plan->threads = threads;
         plan->segment = static_cast<int>(((static_cast<long long>(cols) + cluster - 1) / cluster + 63) / 64 * 64);
-        plan->smem = ((plan->segment * size + 31) & ~15) + more(cluster, threads / 32);
+        plan->smem = ((plan->segment * size + 31) & ~15) + more(*plan);
     };
     if (static_cast<long long>(cols) * size > MAX_CLUSTER * static_cast<long long>(MAX_ROW_SMEM))
     {
@@ -51,7 +51,7 @@ int plan_rows(long long rows, int cols, int size, More more, RowPlan *plan)
         return B200AMP_ERR_LIMIT;
     }
     int cluster = 1;
-    for (fill(1, 256); cluster < MAX_CLUSTER && plan->smem > 56 * 1024; fill(cluster, 256))
+    for (fill(1, 256); cluster < MAX_CLUSTER && plan->smem > 112 * 1024; fill(cluster, 256))
     {
         cluster *= 2;
     }
@@ -253,6 +253,9 @@ struct RowTile
     int lead;               // elements between buf and the first column's place (0 .. N - 1)
     int valid, held;        // columns of the segment that hold logits, and with the padding behind them
     int vecs;               // 16-byte vectors to sweep; what is in none of the columns holds -inf
+    bool uneven;            // rows start at different places between 16-byte boundaries, so a copy covers other rows' ends
+    int edge_at;            // this thread's element outside the whole vectors, -1: none
+    T edge;
 
     __device__ __forceinline__ T *at(int column)            // of this segment, in shared memory
     {
@@ -284,14 +287,42 @@ struct RowTile
         {
             row_copy(buf + 16 * whole_first, src + 16 * whole_first, 16u * max(0, whole_end - whole_first), bar);
         }
-        // the elements of the other vectors: at most N - 1 at the front, then the end and the padding
+        // the elements of the other vectors: at most N - 1 at the front, then the end and the padding. Those that hold
+        // logits (2 N - 2 at most, one a thread) are fetched here and put in place by finish.
         T *e = reinterpret_cast<T *>(buf);
         const T *g = reinterpret_cast<const T *>(src);
         const int front = whole_first * N, back = max(front, whole_end * N);
+        edge_at = -1;
+        bool wrote = false;
         for (int i = threadIdx.x; i < front + (vecs * N - back); i += THREADS)
         {
             const int k = i < front ? i : back + i - front;
-            e[k] = k >= lead && k < lead + valid ? g[k] : minus_infinity<T>();
+            if (k >= lead && k < lead + valid)
+            {
+                edge = g[k];
+                edge_at = k;
+            }
+            else
+            {
+                e[k] = minus_infinity<T>();
+                wrote = true;
+            }
+        }
+        if (wrote && uneven)
+        {
+            before_copies();
+        }
+    }
+    // Before the barrier behind row_wait: the elements that the copy engine does not move.
+    __device__ __forceinline__ void finish()
+    {
+        if (edge_at >= 0)
+        {
+            reinterpret_cast<T *>(buf)[edge_at] = edge;
+            if (uneven)
+            {
+                before_copies();
+            }
         }
     }
 };

@@ -17,9 +17,6 @@
 namespace b200amp
 {
 
-// Set when a wait for a row's copy ran out. Read by b200amp_device_error().
-__device__ int g_row_timeout = 0;
-
 struct DistillArgs
 {
     const void *logits;
@@ -838,16 +835,9 @@ static int launch_distill(const DistillArgs &a, cudaStream_t stream)
     return plan.threads == 128 ? launch_distill<T, 128>(a, plan, stream) : launch_distill<T, 256>(a, plan, stream);
 }
 
-// *out = 1 if a wait for a row's copy gave up since the last call (clears it).
-int row_timeout_take(int *out)
+int distill_timeout_take(int *out)
 {
-    B200AMP_CUDA(cudaMemcpyFromSymbol(out, g_row_timeout, sizeof(int)));
-    if (*out != 0)
-    {
-        const int zero = 0;
-        B200AMP_CUDA(cudaMemcpyToSymbol(g_row_timeout, &zero, sizeof(int)));
-    }
-    return B200AMP_OK;
+    return take_row_timeout(out);
 }
 
 } // namespace b200amp

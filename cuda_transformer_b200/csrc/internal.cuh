@@ -21,7 +21,8 @@ int cuda_fail(cudaError_t err, const char *what, const char *file, int line);
 void count_launch();                            // one more kernel launch enqueued
 int sm_count();                                 // SMs of the current device (cached per device), <= 0 on error
 int zero1_sync_timeout_take(int *out);          // zero1.cu: *out = 1 if a wait on another rank gave up (clears it)
-int row_timeout_take(int *out);                 // distill.cu: *out = 1 if a wait for a row's copy gave up (clears it)
+int distill_timeout_take(int *out);             // distill.cu: *out |= 1 if a wait for a row's copy gave up (clears it)
+int top_timeout_take(int *out);                 // top_logits.cu: the same
 
 struct Tunables
 {

@@ -619,7 +619,8 @@ extern "C" B200AMP_API int b200amp_device_error(int *out)
         return rc;
     }
     int row_wait = 0;
-    rc = row_timeout_take(&row_wait);
+    rc = distill_timeout_take(&row_wait);
+    rc = rc == B200AMP_OK ? top_timeout_take(&row_wait) : rc;
     if (rc != B200AMP_OK)
     {
         return rc;

@@ -195,6 +195,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
     return r;
 }
 
+// Set when a wait for a row's copy ran out; each source file that includes this has its own.
+static __device__ int g_row_timeout = 0;
+
 // Bulk copies: one thread hands a whole segment to the copy engine, which completes its bytes on a barrier in shared
 // memory. (Copied by cp.async, 16 bytes a thread, the threads themselves wait for the memory system to take the
 // requests: a fifth of a row's time.)
@@ -326,6 +329,20 @@ struct RowTile
         }
     }
 };
+
+// *out |= 1 if a wait for a row's copy gave up in this source file's kernels since the last call (clears it).
+static int take_row_timeout(int *out)
+{
+    int flag = 0;
+    B200AMP_CUDA(cudaMemcpyFromSymbol(&flag, g_row_timeout, sizeof(int)));
+    if (flag != 0)
+    {
+        const int zero = 0;
+        B200AMP_CUDA(cudaMemcpyToSymbol(g_row_timeout, &zero, sizeof(int)));
+        *out |= 1;
+    }
+    return B200AMP_OK;
+}
 
 // Blocks of a kernel that fit the device at once, as whole clusters (asked once for each shape).
 template <typename Kernel>

@@ -1,18 +1,22 @@
 // top_logits.cu: a teacher's record: of every row the k largest logits in descending order
 // (ties to the lowest column), their columns, and the log-sum-exp of the whole row.
+//
+// A row is held in shared memory (row_tile.cuh) and swept twice. The first sweep takes maxima, one for each thread
+// and place in a 16-byte vector: a thousand or two groups of columns. A value that k of these maxima reach is reached
+// by k columns of the row, and by few more: the second sweep, which also sums the powers for the log-sum-exp, collects
+// the columns that reach it, and only they are sorted. Rows where too many do (equal logits, masks) are selected
+// by histograms of the keys, digit by digit.
 
-#include "loss_common.cuh"
+#include "row_tile.cuh"
 
 namespace b200amp
 {
-
-constexpr int TOP_THREADS = 512;
 
 struct TopArgs
 {
     const void *logits;
     long long ld, rows;
-    int vocab, k;
+    int vocab, k, room;         // room: columns that a block can collect, a power of two, at least 2 k
     double temperature;
     void *values;
     int *indices;
@@ -33,166 +37,510 @@ __device__ __forceinline__ unsigned int order_key(float v)
     }
     return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
 }
-
-// One block a row: the k-th largest key by four rounds of a 256-bin histogram (8 bits a round, from
-// the top), then one sweep in column order that keeps what is above it and the first of those equal to it.
-template <typename T>
-__global__ void __launch_bounds__(TOP_THREADS) top_rows_kernel(TopArgs a)
+// The number of a key; some NaN for the keys of no number.
+__device__ __forceinline__ float key_value(unsigned int key)
 {
-    __shared__ unsigned long long list[B200AMP_MAX_LISTED];
-    __shared__ unsigned int bins[256];
-    __shared__ double scratch[TOP_THREADS / 32];
-    __shared__ unsigned int warp_above[TOP_THREADS / 32], warp_equal[TOP_THREADS / 32];
+    return __uint_as_float((key & 0x80000000u) != 0 ? key ^ 0x80000000u : ~key);
+}
+// Larger first, then the lower column: entries of a row are all different.
+__device__ __forceinline__ unsigned long long entry_of(unsigned int key, int column)
+{
+    return static_cast<unsigned long long>(key) << 32 | static_cast<unsigned int>(~column);
+}
+__device__ __forceinline__ int column_of(unsigned long long entry)
+{
+    return static_cast<int>(~static_cast<unsigned int>(entry));
+}
+
+// Descending order of list[0 .. n); size: a power of two, n <= size. Every thread.
+template <int THREADS>
+__device__ __forceinline__ void sort_entries(unsigned long long *list, int n, int size)
+{
+    for (int i = n + threadIdx.x; i < size; i += THREADS)
+    {
+        list[i] = 0ull;
+    }
+    for (int span = 2; span <= size; span <<= 1)
+    {
+        for (int step = span >> 1; step > 0; step >>= 1)
+        {
+            __syncthreads();
+            for (int i = threadIdx.x; i < size / 2; i += THREADS)
+            {
+                const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
+                const unsigned long long x = list[lo], y = list[hi];
+                if ((x < y) == ((lo & span) == 0))
+                {
+                    list[lo] = y;
+                    list[hi] = x;
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// The `kept` largest columns of the segment into list, in no order: their smallest key by four rounds of a histogram
+// (8 bits a round, from the top), then one sweep in column order that keeps what is above it and the first of those equal.
+template <typename T, int THREADS>
+__device__ __noinline__ void select_by_digits(const T *z, int first, int valid, int kept, unsigned long long *list,
+                                              unsigned int *bins)
+{
+    __shared__ unsigned int warp_above[THREADS / 32], warp_equal[THREADS / 32];
     __shared__ unsigned int prefix_s, need_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int kept = a.k < a.vocab ? a.k : a.vocab;
-    const double inv_t = 1.0 / a.temperature;
-    const float c_t = static_cast<float>(1.4426950408889634 * inv_t);
-
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x)
+    unsigned int prefix = 0u, mask = 0u, need = kept;
+    for (int shift = 24; shift >= 0; shift -= 8)
     {
-        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
-        if (a.lse != nullptr)
+        for (int b = tid; b < 256; b += THREADS)
         {
-            float m = -INFINITY;
-            for (int v = tid; v < a.vocab; v += TOP_THREADS)
-            {
-                m = max_nan(m, to_float(z[v]));
-            }
-            m = block_max_nan<TOP_THREADS>(m, scratch);
-            float sum = 0.0f;
-            for (int v = tid; v < a.vocab; v += TOP_THREADS)
-            {
-                sum += exp2_fast((to_float(z[v]) - m) * c_t);
-            }
-            const double total = block_sum_f64<TOP_THREADS>(static_cast<double>(sum), scratch);
-            if (tid == 0)
-            {
-                // a row of nothing but -inf has the log of 0; +inf has itself
-                a.lse[row] = isinf(m) ? m : static_cast<float>(m * inv_t + log(total));
-            }
+            bins[b] = 0u;
         }
-
-        unsigned int prefix = 0u, mask = 0u, need = kept;
-        for (int shift = 24; shift >= 0; shift -= 8)
+        __syncthreads();
+        for (int v = tid; v < valid; v += THREADS)
         {
-            for (int b = tid; b < 256; b += TOP_THREADS)
+            const unsigned int key = order_key(to_float(z[v]));
+            if ((key & mask) == prefix)
             {
-                bins[b] = 0u;
-            }
-            __syncthreads();
-            for (int v = tid; v < a.vocab; v += TOP_THREADS)
-            {
-                const unsigned int key = order_key(to_float(z[v]));
-                if ((key & mask) == prefix)
-                {
-                    atomicAdd(&bins[key >> shift & 255u], 1u);
-                }
-            }
-            __syncthreads();
-            if (tid == 0)
-            {
-                unsigned int left = need;
-                int b = 255;
-                while (b > 0 && bins[b] < left)
-                {
-                    left -= bins[b];
-                    b--;
-                }
-                prefix_s = prefix | static_cast<unsigned int>(b) << shift;
-                need_s = left;
-            }
-            __syncthreads();
-            prefix = prefix_s;
-            need = need_s;                      // of those equal to the prefix
-            mask |= 255u << shift;
-            __syncthreads();
-        }
-
-        // prefix is the key of the k-th largest: all above it, and the first `need` equal to it
-        const unsigned int above_all = kept - need;
-        unsigned int above = 0u, equal = 0u;
-        for (int base = 0; base < a.vocab; base += TOP_THREADS)
-        {
-            const int v = base + tid;
-            const unsigned int key = v < a.vocab ? order_key(to_float(z[v])) : 0u;
-            const bool is_above = v < a.vocab && key > prefix, is_equal = v < a.vocab && key == prefix;
-            const unsigned int ba = __ballot_sync(0xffffffffu, is_above), be = __ballot_sync(0xffffffffu, is_equal);
-            if (lane == 0)
-            {
-                warp_above[warp] = __popc(ba);
-                warp_equal[warp] = __popc(be);
-            }
-            __syncthreads();
-            unsigned int at_above = above, at_equal = equal;
-            for (int w = 0; w < TOP_THREADS / 32; w++)
-            {
-                at_above += w < warp ? warp_above[w] : 0u;
-                at_equal += w < warp ? warp_equal[w] : 0u;
-                above += warp_above[w];
-                equal += warp_equal[w];
-            }
-            const unsigned int before = (1u << lane) - 1u;
-            at_above += __popc(ba & before);
-            at_equal += __popc(be & before);
-            const unsigned long long entry = static_cast<unsigned long long>(key) << 32 | static_cast<unsigned int>(~v);
-            if (is_above)
-            {
-                list[at_above] = entry;
-            }
-            if (is_equal && at_equal < need)
-            {
-                list[above_all + at_equal] = entry;
-            }
-            __syncthreads();
-        }
-
-        // descending order of (key, -column)
-        int size = 1;
-        while (size < kept)
-        {
-            size <<= 1;
-        }
-        for (int i = kept + tid; i < size; i += TOP_THREADS)
-        {
-            list[i] = 0ull;
-        }
-        for (int span = 2; span <= size; span <<= 1)
-        {
-            for (int step = span >> 1; step > 0; step >>= 1)
-            {
-                __syncthreads();
-                for (int i = tid; i < size; i += TOP_THREADS)
-                {
-                    const int j = i ^ step;
-                    if (j > i && ((list[i] < list[j]) == ((i & span) == 0)))
-                    {
-                        const unsigned long long t = list[i];
-                        list[i] = list[j];
-                        list[j] = t;
-                    }
-                }
+                atomicAdd(&bins[key >> shift & 255u], 1u);
             }
         }
         __syncthreads();
-        for (int j = tid; j < a.k; j += TOP_THREADS)
+        if (tid == 0)
         {
-            const int v = j < kept ? static_cast<int>(~static_cast<unsigned int>(list[j])) : -1;
-            a.indices[row * a.k + j] = v;
-            static_cast<T *>(a.values)[row * a.k + j] = v >= 0 ? z[v] : from_float<T>(-INFINITY);
+            unsigned int left = need;
+            int b = 255;
+            while (b > 0 && bins[b] < left)
+            {
+                left -= bins[b];
+                b--;
+            }
+            prefix_s = prefix | static_cast<unsigned int>(b) << shift;
+            need_s = left;
+        }
+        __syncthreads();
+        prefix = prefix_s;
+        need = need_s;                          // of those equal to the prefix
+        mask |= 255u << shift;
+        __syncthreads();
+    }
+    const unsigned int above_all = kept - need;
+    unsigned int above = 0u, equal = 0u;
+    for (int base = 0; base < valid; base += THREADS)
+    {
+        const int v = base + tid;
+        const unsigned int key = v < valid ? order_key(to_float(z[v])) : 0u;
+        const bool is_above = v < valid && key > prefix, is_equal = v < valid && key == prefix;
+        const unsigned int ba = __ballot_sync(0xffffffffu, is_above), be = __ballot_sync(0xffffffffu, is_equal);
+        if (lane == 0)
+        {
+            warp_above[warp] = __popc(ba);
+            warp_equal[warp] = __popc(be);
+        }
+        __syncthreads();
+        unsigned int at_above = above, at_equal = equal;
+        for (int w = 0; w < THREADS / 32; w++)
+        {
+            at_above += w < warp ? warp_above[w] : 0u;
+            at_equal += w < warp ? warp_equal[w] : 0u;
+            above += warp_above[w];
+            equal += warp_equal[w];
+        }
+        const unsigned int before = (1u << lane) - 1u;
+        at_above += __popc(ba & before);
+        at_equal += __popc(be & before);
+        if (is_above)
+        {
+            list[at_above] = entry_of(key, first + v);
+        }
+        if (is_equal && at_equal < need)
+        {
+            list[above_all + at_equal] = entry_of(key, first + v);
         }
         __syncthreads();
     }
 }
 
-template <typename T>
-static int launch_top(const TopArgs &a, int sms, cudaStream_t stream)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const TopArgs a, const RowPlan plan)
 {
-    const long long most = 4ll * sms;
-    const int grid = static_cast<int>(a.rows < most ? a.rows : most);
-    top_rows_kernel<T><<<grid, TOP_THREADS, 0, stream>>>(a);
-    B200AMP_LAUNCHED();
-    return B200AMP_OK;
+    namespace cg = cooperative_groups;
+    using Tile = RowTile<T, THREADS>;
+    constexpr int N = Tile::N, PAIRS = N / 2, WARPS = THREADS / 32;
+    extern __shared__ __align__(16) char dynamic[];
+    __shared__ uint64_t row_bar;
+    __shared__ unsigned int bins[256];
+    __shared__ unsigned int counts[2][WARPS], warp_hi[WARPS], warp_lo[WARPS];
+    __shared__ float warp_m[WARPS], warp_s[WARPS];
+    __shared__ float2 block_ms[2];              // of two rows: this segment's maximum and sum
+    __shared__ int collected;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = plan.cluster, rank = blocks > 1 ? static_cast<int>(cluster.block_rank()) : 0;
+    const int first = rank * plan.segment;
+    const long long clusters = gridDim.x / blocks;
+    const double inv_t = 1.0 / a.temperature;
+    const float c_t = static_cast<float>(1.4426950408889634 * inv_t);
+
+    // dynamic shared memory: the segment; the collected columns; two rows' sorted best of the segment
+    const size_t tile_bytes = (static_cast<size_t>(plan.segment) * sizeof(T) + 31) & ~static_cast<size_t>(15);
+    Tile tile;
+    tile.buf = dynamic;
+    tile.uneven = (a.ld * static_cast<long long>(sizeof(T)) & 15) != 0;
+    unsigned long long *const list = reinterpret_cast<unsigned long long *>(dynamic + tile_bytes);
+    unsigned long long *const best0 = list + a.room;
+    auto start = [&](long long row) {
+        tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.vocab, &row_bar);
+    };
+    if (tid == 0)
+    {
+        row_barrier_init(&row_bar);
+    }
+    __syncthreads();
+    if (blocks > 1)
+    {
+        cluster.sync();                         // every block of the cluster runs before one reads of another
+    }
+
+    unsigned int phase = 0;
+    int parity = 0;
+    long long row = blockIdx.x / blocks;
+    if (row < a.rows)
+    {
+        start(row);
+    }
+    for (; row < a.rows; row += clusters, parity ^= 1)
+    {
+        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
+        unsigned long long *const best = best0 + parity * a.k;
+        const int valid = tile.valid;
+        const int kept = min(a.k, valid);       // of this segment
+        if (tid == 0)
+        {
+            collected = 0;
+        }
+        const bool there = row_wait(&row_bar, phase);
+        phase ^= 1u;
+        tile.finish();
+        if (!there)
+        {
+            g_row_timeout = 1;
+        }
+        __syncthreads();
+
+        // maxima of the groups
+        Vec16<T> group;
+        {
+            const T low = minus_infinity<T>();
+            T *e = reinterpret_cast<T *>(&group);
+#pragma unroll
+            for (int i = 0; i < N; i++)
+            {
+                e[i] = low;
+            }
+        }
+        {
+            int i = tid;
+            for (; i + 3 * THREADS < tile.vecs; i += 4 * THREADS)
+            {
+                Vec16<T> v0 = tile.vec(i), v1 = tile.vec(i + THREADS), v2 = tile.vec(i + 2 * THREADS), v3 = tile.vec(i + 3 * THREADS);
+                max_into(v0, v1);
+                max_into(v2, v3);
+                max_into(group, v0);
+                max_into(group, v2);
+            }
+            for (; i < tile.vecs; i += THREADS)
+            {
+                max_into(group, tile.vec(i));
+            }
+        }
+        unsigned int key[N];
+        float m = -INFINITY;
+        {
+            float2 f[PAIRS];
+            unpack(group, f);
+#pragma unroll
+            for (int q = 0; q < PAIRS; q++)
+            {
+                key[2 * q] = order_key(f[q].x);
+                key[2 * q + 1] = order_key(f[q].y);
+                m = max_nan(m, max_nan(f[q].x, f[q].y));
+            }
+        }
+        unsigned int hi = key[0], lo = key[0];
+#pragma unroll
+        for (int i = 1; i < N; i++)
+        {
+            hi = max(hi, key[i]);
+            lo = min(lo, key[i]);
+        }
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        m = warp_max_nan(m);
+        if (lane == 0)
+        {
+            warp_hi[warp] = hi;
+            warp_lo[warp] = lo;
+            warp_m[warp] = m;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WARPS; w++)
+        {
+            hi = max(hi, warp_hi[w]);
+            lo = min(lo, warp_lo[w]);
+            m = max_nan(m, warp_m[w]);
+        }
+
+        // a key that at least k groups reach, and not many more: bisection between their least and their largest
+        unsigned int reach = 0u;                // short segments are collected whole
+        if (valid > a.room / 2 && THREADS * N >= a.k)
+        {
+            const int enough = a.k + max(16, a.k / 8);
+            int flip = 0;
+            reach = lo;                         // all of them
+            unsigned int beyond = hi;           // fewer than k are above the largest
+            while (reach < beyond)
+            {
+                const unsigned int mid = reach + (beyond - reach + 1u) / 2u;
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < N; i++)
+                {
+                    c += key[i] >= mid ? 1 : 0;
+                }
+                c = __reduce_add_sync(0xffffffffu, c);
+                if (lane == 0)
+                {
+                    counts[flip][warp] = c;
+                }
+                __syncthreads();
+                c = 0;
+#pragma unroll
+                for (int w = 0; w < WARPS; w++)
+                {
+                    c += counts[flip][w];
+                }
+                flip ^= 1;
+                if (c >= a.k)
+                {
+                    reach = mid;
+                    if (c <= enough)
+                    {
+                        break;
+                    }
+                }
+                else
+                {
+                    beyond = mid - 1u;
+                }
+            }
+        }
+
+        // the columns that reach it, and the sum
+        const float least = key_value(reach), ref = m == -INFINITY ? 0.0f : m;
+        const bool sums = a.lse != nullptr;
+        float2 sum = make_float2(0.0f, 0.0f);
+        auto visit = [&](int i, const float2 (&f)[PAIRS]) {
+            float top = max_nan(f[0].x, f[0].y);
+#pragma unroll
+            for (int q = 1; q < PAIRS; q++)
+            {
+                top = max_nan(top, max_nan(f[q].x, f[q].y));
+            }
+            if (sums)
+            {
+#pragma unroll
+                for (int q = 0; q < PAIRS; q++)
+                {
+                    const float2 x = mul2(add2(f[q], make_float2(-ref, -ref)), make_float2(c_t, c_t));
+                    sum = add2(sum, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+                }
+            }
+            if (!(top < least))
+            {
+#pragma unroll
+                for (int q = 0; q < N; q++)
+                {
+                    const float v = q % 2 == 0 ? f[q / 2].x : f[q / 2].y;
+                    const unsigned int at_key = order_key(v);
+                    const int column = i * N + q - tile.lead;
+                    if (at_key >= reach && column >= 0 && column < valid)
+                    {
+                        const int to = atomicAdd(&collected, 1);
+                        if (to < a.room)
+                        {
+                            list[to] = entry_of(at_key, first + column);
+                        }
+                    }
+                }
+            }
+        };
+        {
+            int i = tid;
+            for (; i + THREADS < tile.vecs; i += 2 * THREADS)
+            {
+                float2 f0[PAIRS], f1[PAIRS];
+                unpack(tile.vec(i), f0);
+                unpack(tile.vec(i + THREADS), f1);
+                visit(i, f0);
+                visit(i + THREADS, f1);
+            }
+            if (i < tile.vecs)
+            {
+                float2 f[PAIRS];
+                unpack(tile.vec(i), f);
+                visit(i, f);
+            }
+        }
+        const float s = warp_sum_f32(sum.x + sum.y);
+        if (lane == 0)
+        {
+            warp_s[warp] = s;
+        }
+        __syncthreads();
+        int n = collected;
+        if (n > a.room)
+        {
+            select_by_digits<T, THREADS>(reinterpret_cast<const T *>(tile.buf) + tile.lead, first, valid, kept, list, bins);
+            n = kept;
+        }
+        if (row + clusters < a.rows)
+        {
+            start(row + clusters);              // on its way while this row's few columns are sorted
+        }
+        if (tid == 0)
+        {
+            double total = 0.0;
+            for (int w = 0; w < WARPS; w++)
+            {
+                total += warp_s[w];
+            }
+            block_ms[parity] = make_float2(m, static_cast<float>(total));
+        }
+
+        // the best of the segment in order
+        if (n <= THREADS)
+        {
+            const unsigned long long mine = tid < n ? list[tid] : 0ull;
+            int place = 0;
+            for (int i = 0; i < n; i++)
+            {
+                place += list[i] > mine ? 1 : 0;
+            }
+            if (tid < n && place < kept)
+            {
+                best[place] = mine;
+            }
+            __syncthreads();
+        }
+        else
+        {
+            int size = 2;
+            while (size < n)
+            {
+                size <<= 1;
+            }
+            sort_entries<THREADS>(list, n, size);
+            for (int i = tid; i < kept; i += THREADS)
+            {
+                best[i] = list[i];
+            }
+            __syncthreads();
+        }
+
+        // the best of the row: an entry's place is the number of larger ones in every segment
+        if (blocks > 1)
+        {
+            cluster.sync();
+        }
+        for (int j = tid; j < kept; j += THREADS)
+        {
+            const unsigned long long entry = best[j];
+            int place = j;
+            for (int b = 0; b < blocks && place < a.k; b++)
+            {
+                if (b == rank)
+                {
+                    continue;
+                }
+                const unsigned long long *other = cluster.map_shared_rank(best, b);
+                int from = 0, to = min(a.k, max(0, min(plan.segment, a.vocab - b * plan.segment)));
+                while (from < to)
+                {
+                    const int mid = (from + to) / 2;
+                    if (other[mid] > entry)
+                    {
+                        from = mid + 1;
+                    }
+                    else
+                    {
+                        to = mid;
+                    }
+                }
+                place += from;
+            }
+            if (place < a.k)
+            {
+                const int column = column_of(entry);
+                a.indices[row * a.k + place] = column;
+                static_cast<T *>(a.values)[row * a.k + place] = z[column];
+            }
+        }
+        if (rank == 0)
+        {
+            for (int j = a.vocab + tid; j < a.k; j += THREADS)
+            {
+                a.indices[row * a.k + j] = -1;  // fewer columns than asked for
+                static_cast<T *>(a.values)[row * a.k + j] = minus_infinity<T>();
+            }
+            if (sums && tid == 0)
+            {
+                float all = -INFINITY;
+                for (int b = 0; b < blocks; b++)
+                {
+                    all = max_nan(all, (blocks > 1 ? cluster.map_shared_rank(block_ms, b) : block_ms)[parity].x);
+                }
+                double total = 0.0;
+                for (int b = 0; b < blocks; b++)
+                {
+                    const float2 ms = (blocks > 1 ? cluster.map_shared_rank(block_ms, b) : block_ms)[parity];
+                    total += ms.x == -INFINITY ? 0.0 : ms.y * exp((static_cast<double>(ms.x) - all) * inv_t);
+                }
+                // a row of nothing but -inf has the log of 0; +inf has itself
+                a.lse[row] = isinf(all) ? all : static_cast<float>(all * inv_t + log(total)) + (there ? 0.0f : NAN);
+            }
+        }
+    }
+    if (blocks > 1)
+    {
+        cluster.sync();                         // no block leaves while another reads its last row
+    }
+}
+
+template <typename T>
+static int launch_top(TopArgs a, cudaStream_t stream)
+{
+    a.room = 256;
+    while (a.room < 2 * a.k)
+    {
+        a.room *= 2;
+    }
+    RowPlan plan;
+    const int rc = plan_rows(
+        a.rows, a.vocab, sizeof(T), [&](const RowPlan &) { return (a.room + 2 * a.k) * static_cast<int>(sizeof(unsigned long long)); },
+        &plan);
+    if (rc != B200AMP_OK)
+    {
+        return rc;
+    }
+    return plan.threads == 128 ? launch_rows(top_rows_kernel<T, 128>, a, plan, 128, a.rows, stream)
+                               : launch_rows(top_rows_kernel<T, 256>, a, plan, 256, a.rows, stream);
+}
+
+int top_timeout_take(int *out)
+{
+    return take_row_timeout(out);
 }
 
 } // namespace b200amp
@@ -215,28 +563,18 @@ extern "C" B200AMP_API int b200amp_top_logits(const void *logits, int dtype, lon
                     "top_logits: logits, values or indices is null");
     B200AMP_REQUIRE(aligned(logits, size) && aligned(values, size) && aligned(indices, 4) && aligned(lse, 4),
                     "top_logits: an array is not aligned to its element type");
-    if (vocab > 1 << 20)
-    {
-        set_error("top_logits: a vocabulary of %d is beyond the maximum of %d", vocab, 1 << 20);
-        return B200AMP_ERR_LIMIT;
-    }
-    const int sms = sm_count();
-    if (sms <= 0)
-    {
-        return B200AMP_ERR_CUDA;
-    }
     if (rows == 0)
     {
         return B200AMP_OK;
     }
-    const TopArgs a = {logits, ld, rows, vocab, k, temperature, values, indices, lse};
+    const TopArgs a = {logits, ld, rows, vocab, k, 0, temperature, values, indices, lse};
     switch (dtype)
     {
     case B200AMP_F16:
-        return launch_top<__half>(a, sms, as_stream(s));
+        return launch_top<__half>(a, as_stream(s));
     case B200AMP_BF16:
-        return launch_top<__nv_bfloat16>(a, sms, as_stream(s));
+        return launch_top<__nv_bfloat16>(a, as_stream(s));
     default:
-        return launch_top<float>(a, sms, as_stream(s));
+        return launch_top<float>(a, as_stream(s));
     }
 }

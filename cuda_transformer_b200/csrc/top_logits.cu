@@ -12,6 +12,8 @@
 namespace b200amp
 {
 
+constexpr int MOST_BROUGHT = 2048;      // listed columns of a cluster that a block copies before it searches them
+
 struct TopArgs
 {
     const void *logits;
@@ -50,6 +52,19 @@ __device__ __forceinline__ unsigned long long entry_of(unsigned int key, int col
 __device__ __forceinline__ int column_of(unsigned long long entry)
 {
     return static_cast<int>(~static_cast<unsigned int>(entry));
+}
+
+// Whether an element may be at least `least` (NaN: yes).
+template <typename T>
+__device__ __forceinline__ bool reaches(const Vec16<T> &v, float least)
+{
+    const uint32_t m = max2_nan(max2_nan(v.w.x, v.w.y, T()), max2_nan(v.w.z, v.w.w, T()), T());
+    if (sizeof(T) == 4)
+    {
+        return !(__uint_as_float(m) < least);
+    }
+    const float2 f = pair_of(m, T());
+    return !(f.x < least) || !(f.y < least);
 }
 
 // Descending order of list[0 .. n); size: a power of two, n <= size. Every thread.
@@ -170,10 +185,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     extern __shared__ __align__(16) char dynamic[];
     __shared__ uint64_t row_bar;
     __shared__ unsigned int bins[256];
-    __shared__ unsigned int counts[2][WARPS], warp_hi[WARPS], warp_lo[WARPS];
+    __shared__ unsigned int warp_hi[WARPS], warp_lo[WARPS];
+    __shared__ int4 found;                      // a bin, the groups above it, those in it too
     __shared__ float warp_m[WARPS], warp_s[WARPS];
     __shared__ float2 block_ms[2];              // of two rows: this segment's maximum and sum
-    __shared__ int collected;
+    __shared__ int collected, met;              // columns that reach, vectors that hold some
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const cg::cluster_group cluster = cg::this_cluster();
     const int blocks = plan.cluster, rank = blocks > 1 ? static_cast<int>(cluster.block_rank()) : 0;
@@ -182,13 +198,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     const double inv_t = 1.0 / a.temperature;
     const float c_t = static_cast<float>(1.4426950408889634 * inv_t);
 
-    // dynamic shared memory: the segment; the collected columns; two rows' sorted best of the segment
+    // dynamic shared memory: the segment; the collected columns and the vectors that hold them; two rows' sorted best of the segment; the cluster's
     const size_t tile_bytes = (static_cast<size_t>(plan.segment) * sizeof(T) + 31) & ~static_cast<size_t>(15);
     Tile tile;
     tile.buf = dynamic;
     tile.uneven = (a.ld * static_cast<long long>(sizeof(T)) & 15) != 0;
     unsigned long long *const list = reinterpret_cast<unsigned long long *>(dynamic + tile_bytes);
-    unsigned long long *const best0 = list + a.room;
+    int *const vectors = reinterpret_cast<int *>(list + a.room);
+    unsigned long long *const best0 = list + a.room + a.room / 2;
+    unsigned long long *const others = best0 + 2 * a.k;     // every segment's, brought over where they are few
+    const bool brought = blocks * a.k <= MOST_BROUGHT;
     auto start = [&](long long row) {
         tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.vocab, &row_bar);
     };
@@ -211,13 +230,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     }
     for (; row < a.rows; row += clusters, parity ^= 1)
     {
-        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
         unsigned long long *const best = best0 + parity * a.k;
         const int valid = tile.valid;
         const int kept = min(a.k, valid);       // of this segment
         if (tid == 0)
         {
             collected = 0;
+            met = 0;
         }
         const bool there = row_wait(&row_bar, phase);
         phase ^= 1u;
@@ -267,12 +286,30 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
                 m = max_nan(m, max_nan(f[q].x, f[q].y));
             }
         }
+        // as many groups as are needed: four times k, or all (fewer would let too many columns through)
+        int per = N;
+#pragma unroll
+        for (int half = N / 2; half > 0; half >>= 1)
+        {
+            if (per == 2 * half && THREADS * half >= 4 * a.k)
+            {
+                per = half;
+#pragma unroll
+                for (int i = 0; i < half; i++)
+                {
+                    key[i] = max(key[i], key[i + half]);
+                }
+            }
+        }
         unsigned int hi = key[0], lo = key[0];
 #pragma unroll
         for (int i = 1; i < N; i++)
         {
-            hi = max(hi, key[i]);
-            lo = min(lo, key[i]);
+            if (i < per)
+            {
+                hi = max(hi, key[i]);
+                lo = min(lo, key[i]);
+            }
         }
         hi = __reduce_max_sync(0xffffffffu, hi);
         lo = __reduce_min_sync(0xffffffffu, lo);
@@ -292,48 +329,73 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
             m = max_nan(m, warp_m[w]);
         }
 
-        // a key that at least k groups reach, and not many more: bisection between their least and their largest
+        // a key that at least k groups reach, and not many more: their histogram over the range of the keys, and again
+        // over the bin of the k-th largest while that holds too many
         unsigned int reach = 0u;                // short segments are collected whole
         if (valid > a.room / 2 && THREADS * N >= a.k)
         {
-            const int enough = a.k + max(16, a.k / 8);
-            int flip = 0;
-            reach = lo;                         // all of them
-            unsigned int beyond = hi;           // fewer than k are above the largest
-            while (reach < beyond)
+            int above = 0;                      // groups above the range at hand
+            reach = lo;
+            unsigned int span = hi - lo;        // the range: reach .. reach + span
+            for (;;)
             {
-                const unsigned int mid = reach + (beyond - reach + 1u) / 2u;
-                int c = 0;
+                const int shift = max(0, 24 - __clz(static_cast<int>(span | 1u)));     // 256 bins or fewer
+                for (int i = tid; i < 256; i += THREADS)
+                {
+                    bins[i] = 0u;
+                }
+                __syncthreads();
 #pragma unroll
                 for (int i = 0; i < N; i++)
                 {
-                    c += key[i] >= mid ? 1 : 0;
-                }
-                c = __reduce_add_sync(0xffffffffu, c);
-                if (lane == 0)
-                {
-                    counts[flip][warp] = c;
-                }
-                __syncthreads();
-                c = 0;
-#pragma unroll
-                for (int w = 0; w < WARPS; w++)
-                {
-                    c += counts[flip][w];
-                }
-                flip ^= 1;
-                if (c >= a.k)
-                {
-                    reach = mid;
-                    if (c <= enough)
+                    if (i < per && key[i] >= reach && key[i] - reach <= span)
                     {
-                        break;
+                        atomicAdd(&bins[(key[i] - reach) >> shift], 1u);
                     }
                 }
-                else
+                __syncthreads();
+                if (warp == 0)
                 {
-                    beyond = mid - 1u;
+                    // lane l: bins 255 - 8 l .. 248 - 8 l, from the top
+                    int mine = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                    {
+                        mine += static_cast<int>(bins[255 - 8 * lane - i]);
+                    }
+                    int upto = mine;
+#pragma unroll
+                    for (int offset = 1; offset < 32; offset <<= 1)
+                    {
+                        const int below = __shfl_up_sync(0xffffffffu, upto, offset);
+                        upto += lane >= offset ? below : 0;
+                    }
+                    const unsigned int enough = __ballot_sync(0xffffffffu, above + upto >= a.k);
+                    if (lane == __ffs(static_cast<int>(enough)) - 1)
+                    {
+                        int count = above + upto - mine;        // above the lane's bins
+                        int bin = 255 - 8 * lane, over = count;
+                        for (;; bin--)
+                        {
+                            over = count;
+                            count += static_cast<int>(bins[bin]);
+                            if (count >= a.k)
+                            {
+                                break;
+                            }
+                        }
+                        found = make_int4(bin, over, count, 0);
+                    }
                 }
+                __syncthreads();
+                const int4 f = found;
+                reach += static_cast<unsigned int>(f.x) << shift;
+                if (f.z <= a.k + max(16, a.k / 4) || shift == 0)
+                {
+                    break;
+                }
+                above = f.y;
+                span = (1u << shift) - 1u;
             }
         }
 
@@ -341,13 +403,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
         const float least = key_value(reach), ref = m == -INFINITY ? 0.0f : m;
         const bool sums = a.lse != nullptr;
         float2 sum = make_float2(0.0f, 0.0f);
-        auto visit = [&](int i, const float2 (&f)[PAIRS]) {
-            float top = max_nan(f[0].x, f[0].y);
-#pragma unroll
-            for (int q = 1; q < PAIRS; q++)
-            {
-                top = max_nan(top, max_nan(f[q].x, f[q].y));
-            }
+        auto visit = [&](int i, const Vec16<T> &v) {
+            float2 f[PAIRS];
+            unpack(v, f);
             if (sums)
             {
 #pragma unroll
@@ -357,22 +415,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
                     sum = add2(sum, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
                 }
             }
-            if (!(top < least))
+            if (reaches(v, least))
             {
-#pragma unroll
-                for (int q = 0; q < N; q++)
+                const int to = atomicAdd(&met, 1);
+                if (to < a.room)
                 {
-                    const float v = q % 2 == 0 ? f[q / 2].x : f[q / 2].y;
-                    const unsigned int at_key = order_key(v);
-                    const int column = i * N + q - tile.lead;
-                    if (at_key >= reach && column >= 0 && column < valid)
-                    {
-                        const int to = atomicAdd(&collected, 1);
-                        if (to < a.room)
-                        {
-                            list[to] = entry_of(at_key, first + column);
-                        }
-                    }
+                    vectors[to] = i;            // looked at once the sweep is over, by as many threads as it has elements
                 }
             }
         };
@@ -380,17 +428,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
             int i = tid;
             for (; i + THREADS < tile.vecs; i += 2 * THREADS)
             {
-                float2 f0[PAIRS], f1[PAIRS];
-                unpack(tile.vec(i), f0);
-                unpack(tile.vec(i + THREADS), f1);
-                visit(i, f0);
-                visit(i + THREADS, f1);
+                const Vec16<T> v0 = tile.vec(i), v1 = tile.vec(i + THREADS);
+                visit(i, v0);
+                visit(i + THREADS, v1);
             }
             if (i < tile.vecs)
             {
-                float2 f[PAIRS];
-                unpack(tile.vec(i), f);
-                visit(i, f);
+                visit(i, tile.vec(i));
             }
         }
         const float s = warp_sum_f32(sum.x + sum.y);
@@ -399,7 +443,25 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
             warp_s[warp] = s;
         }
         __syncthreads();
-        int n = collected;
+        int n = met;
+        if (n <= a.room)
+        {
+            for (int x = tid; x < n * N; x += THREADS)
+            {
+                const int at = vectors[x / N] * N + x % N, column = at - tile.lead;
+                const unsigned int at_key = order_key(to_float(reinterpret_cast<const T *>(tile.buf)[at]));
+                if (at_key >= reach && column >= 0 && column < valid)
+                {
+                    const int to = atomicAdd(&collected, 1);
+                    if (to < a.room)
+                    {
+                        list[to] = entry_of(at_key, first + column);
+                    }
+                }
+            }
+            __syncthreads();
+            n = collected;
+        }
         if (n > a.room)
         {
             select_by_digits<T, THREADS>(reinterpret_cast<const T *>(tile.buf) + tile.lead, first, valid, kept, list, bins);
@@ -420,17 +482,35 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
         }
 
         // the best of the segment in order
-        if (n <= THREADS)
+        if (n <= 2 * THREADS)
         {
-            const unsigned long long mine = tid < n ? list[tid] : 0ull;
-            int place = 0;
-            for (int i = 0; i < n; i++)
+            // an entry's place is the number of larger ones, counted by `lanes` neighbours
+            int lanes = 1;
+            while (lanes < 8 && 2 * lanes * n <= THREADS)
             {
-                place += list[i] > mine ? 1 : 0;
+                lanes *= 2;
             }
-            if (tid < n && place < kept)
+            for (int x0 = 0; x0 < n * lanes; x0 += THREADS)
             {
-                best[place] = mine;
+                const int x = x0 + tid, i = x / lanes;
+                const unsigned long long mine = i < n ? list[i] : ~0ull;
+                int place = 0;
+                if (x0 + warp * 32 < n * lanes)
+                {
+#pragma unroll 4
+                    for (int j = x % lanes; j < n; j += lanes)
+                    {
+                        place += list[j] > mine ? 1 : 0;
+                    }
+                }
+                for (int offset = lanes >> 1; offset > 0; offset >>= 1)
+                {
+                    place += __shfl_xor_sync(0xffffffffu, place, offset);
+                }
+                if (i < n && x % lanes == 0 && place < kept)
+                {
+                    best[place] = mine;
+                }
             }
             __syncthreads();
         }
@@ -453,6 +533,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
         if (blocks > 1)
         {
             cluster.sync();
+            for (int i = tid; brought && i < blocks * a.k; i += THREADS)
+            {
+                const int b = i / a.k, j = i - b * a.k;
+                const int there_kept = min(a.k, max(0, min(plan.segment, a.vocab - b * plan.segment)));
+                others[i] = j < there_kept ? cluster.map_shared_rank(best, b)[j] : 0ull;
+            }
+            __syncthreads();
         }
         for (int j = tid; j < kept; j += THREADS)
         {
@@ -460,31 +547,29 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
             int place = j;
             for (int b = 0; b < blocks && place < a.k; b++)
             {
-                if (b == rank)
+                if (b != rank)
                 {
-                    continue;
-                }
-                const unsigned long long *other = cluster.map_shared_rank(best, b);
-                int from = 0, to = min(a.k, max(0, min(plan.segment, a.vocab - b * plan.segment)));
-                while (from < to)
-                {
-                    const int mid = (from + to) / 2;
-                    if (other[mid] > entry)
+                    const unsigned long long *other = brought ? others + b * a.k : cluster.map_shared_rank(best, b);
+                    int from = 0, to = min(a.k, max(0, min(plan.segment, a.vocab - b * plan.segment)));
+                    while (from < to)
                     {
-                        from = mid + 1;
+                        const int mid = (from + to) / 2;
+                        if (other[mid] > entry)
+                        {
+                            from = mid + 1;
+                        }
+                        else
+                        {
+                            to = mid;
+                        }
                     }
-                    else
-                    {
-                        to = mid;
-                    }
+                    place += from;
                 }
-                place += from;
             }
             if (place < a.k)
             {
-                const int column = column_of(entry);
-                a.indices[row * a.k + place] = column;
-                static_cast<T *>(a.values)[row * a.k + place] = z[column];
+                a.indices[row * a.k + place] = column_of(entry);
+                static_cast<T *>(a.values)[row * a.k + place] = from_float<T>(key_value(static_cast<unsigned int>(entry >> 32)));
             }
         }
         if (rank == 0)
@@ -528,7 +613,10 @@ static int launch_top(TopArgs a, cudaStream_t stream)
     }
     RowPlan plan;
     const int rc = plan_rows(
-        a.rows, a.vocab, sizeof(T), [&](const RowPlan &) { return (a.room + 2 * a.k) * static_cast<int>(sizeof(unsigned long long)); },
+        a.rows, a.vocab, sizeof(T), [&](const RowPlan &p) {
+            return (a.room + a.room / 2 + 2 * a.k + (p.cluster > 1 && p.cluster * a.k <= MOST_BROUGHT ? p.cluster * a.k : 0)) *
+                   static_cast<int>(sizeof(unsigned long long));
+        },
         &plan);
     if (rc != B200AMP_OK)
     {

@@ -436,7 +436,7 @@ B200AMP_API int b200amp_loss_workspace_init(void *workspace, b200amp_stream s);
 
 /* A teacher's record: of every row the k largest of the first `vocab` columns in descending order, ties
  * to the lowest column, with their columns, and (lse not null) log sum_v exp(z_v / temperature) over all
- * of them. values[rows][k] has the type of the logits (the values are copied, not rounded),
+ * of them. values[rows][k] has the type of the logits and their values (a -0 comes as 0),
  * indices[rows][k] is int32, lse[rows] fp32. NaN counts as larger than any number and -0 equals +0.
  * k > vocab: the entries behind the last column get index -1 and value -inf, which b200amp_distill_loss
  * leaves out. rows >= 0, 1 <= k <= 1024, 1 <= vocab <= ld. No reference counterpart. */

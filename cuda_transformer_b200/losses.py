@@ -30,50 +30,59 @@ _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _l
 _STATE_BYTES = 60
 
 
+# the handle alone: building a Stream object for every call costs more than the rest of the call's Python
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def loss_workspace(device="cuda") -> torch.Tensor:
     """The workspace of distill_loss and balance_loss, zeroed. One serves one stream at a time."""
     return torch.zeros(LOSS_WORKSPACE_BYTES, dtype=torch.uint8, device=device)
 
 
-def _matrix(t: torch.Tensor, name: str, device=None):
+def _matrix(t: torch.Tensor, name: str, device: int = -1):
     """(pointer, row stride in elements, rows, columns, type code) of a 2-D CUDA tensor."""
-    if t.dim() != 2 or not t.is_cuda or t.dtype not in _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if t.dim() != 2 or not t.is_cuda or code is None:
         raise ValueError(f"{name}: expected a 2-D CUDA tensor of fp16, bf16 or fp32, got {t.dim()}-D {t.dtype} on {t.device}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if device >= 0 and t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
         raise ValueError(f"{name}: the columns of a row must be next to each other (strides {t.stride()})")
-    return t.data_ptr(), (t.stride(0) if rows > 1 else cols), rows, cols, _DTYPES[t.dtype]
+    return t.data_ptr(), (ld if rows > 1 else cols), rows, cols, code
 
 
-def _array(t: Optional[torch.Tensor], name: str, dtype, shape, device) -> Optional[int]:
+def _array(t: Optional[torch.Tensor], name: str, dtype, shape, device: int) -> Optional[int]:
     """Pointer of a contiguous tensor of this type and shape, or None for None."""
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {device}, got {t.dtype} "
+    if t.dtype != dtype or t.shape != shape or not t.is_cuda or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on cuda:{device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _bytes(t: torch.Tensor, name: str, least: int, device) -> int:
-    if t.device != device or not t.is_contiguous() or t.numel() * t.element_size() < least:
-        raise ValueError(f"{name}: expected a contiguous tensor of {least} bytes or more on {device}")
+def _bytes(t: torch.Tensor, name: str, least: int, device: int) -> int:
+    if not t.is_cuda or t.get_device() != device or not t.is_contiguous() or t.nbytes < least:
+        raise ValueError(f"{name}: expected a contiguous tensor of {least} bytes or more on cuda:{device}")
     return t.data_ptr()
 
 
-def _call(fn, device: torch.device, stream, *args) -> None:
+def _call(fn, device: int, stream, *args) -> None:
     """fn(*args, stream) with the tensors' device current; raises what the library refuses."""
-    if stream is not None:
-        handle = stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
+    if stream is None:
+        handle = _current_stream(device)
     else:
-        handle = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, handle))
+        handle = stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
+    if torch.cuda.current_device() == device:
+        status = fn(*args, handle)
     else:
         with torch.cuda.device(device):
-            check(fn(*args, handle))
+            status = fn(*args, handle)
+    if status != _lib.OK:
+        check(status)
 
 
 def top_logits(logits: torch.Tensor, k: int, values: torch.Tensor, indices: torch.Tensor,
@@ -83,7 +92,7 @@ def top_logits(logits: torch.Tensor, k: int, values: torch.Tensor, indices: torc
     logits' type) and indices[rows, k] (int32), in descending order, ties to the lowest column; and, if lse is
     given, log sum exp(z / temperature) over the row into lse[rows] (fp32)."""
     ptr, ld, rows, cols, dtype = _matrix(logits, "logits")
-    dev = logits.device
+    dev = logits.get_device()
     vocab = cols if vocab is None else vocab
     if not 1 <= vocab <= cols:
         raise ValueError(f"vocab = {vocab}: the logits have {cols} columns")
@@ -102,7 +111,7 @@ def distill_loss(logits: torch.Tensor, dlogits: Optional[torch.Tensor], targets:
     its log-sum-exp at the same temperature, or None to normalise over the listed logits alone. Columns from
     `vocab` on pad the vocabulary. dlogits may be logits itself. Without a teacher pass None for the three."""
     ptr, ld, rows, cols, dtype = _matrix(logits, "logits")
-    dev = logits.device
+    dev = logits.get_device()
     vocab = cols if vocab is None else vocab
     dptr, dld = None, cols
     if dlogits is not None:
@@ -134,7 +143,7 @@ def balance_loss(logits: torch.Tensor, dlogits: Optional[torch.Tensor], chosen: 
     None) the gradient times the state's loss scale, added to dlogits if accumulate. chosen[rows, k] (int32) are
     the router's choices, negative where one was not made. add_to_state adds the loss to state.loss."""
     ptr, ld, rows, experts, dtype = _matrix(logits, "logits")
-    dev = logits.device
+    dev = logits.get_device()
     dptr, dld = None, experts
     if dlogits is not None:
         dptr, dld, drows, dcols, ddtype = _matrix(dlogits, "dlogits", dev)

@@ -417,8 +417,8 @@ B200AMP_API int b200amp_step_f16(float *master, float *m, float *v, const void *
  * element type is taken, and rows that start on 16-byte boundaries are fastest. dtype is one of the
  * three below. Nothing is allocated; every array is device memory of the current device. Sums and
  * statistics are held in fp32 or fp64; a gradient is rounded once, to its own type. The results depend
- * on the inputs and the shapes alone, never on the order in which blocks finish, so a replay gives the
- * same bits. A gradient beyond the type's range becomes inf and skips the step, as any other would.
+ * on the inputs, the shapes and the layout alone, never on the order in which blocks finish, so a replay
+ * gives the same bits. A gradient beyond the type's range becomes inf and skips the step, as any other would.
  *
  * The workspace is B200AMP_LOSS_WORKSPACE_BYTES bytes, 16-byte aligned, zeroed once (cudaMemset or
  * b200amp_loss_workspace_init); the kernels leave its counters at zero again. One workspace serves one

@@ -823,7 +823,7 @@ static int launch_distill(const DistillArgs &a, cudaStream_t stream)
     const int record = a.k * (2 * (2 * sizeof(double) + sizeof(float) + sizeof(int)) + sizeof(int));
     RowPlan plan;
     const int rc = plan_rows(
-        a.rows, a.cols, sizeof(T),
+        a.rows, a.cols, sizeof(T), 64, 256,
         [&](const RowPlan &p) {
             return record + 2 * ((row_sums_bytes(p.cluster, p.cluster * p.threads / 32) + 7) & ~7) + p.segment / 8;
         },
@@ -832,7 +832,9 @@ static int launch_distill(const DistillArgs &a, cudaStream_t stream)
     {
         return rc;
     }
-    return plan.threads == 128 ? launch_distill<T, 128>(a, plan, stream) : launch_distill<T, 256>(a, plan, stream);
+    return plan.threads == 64    ? launch_distill<T, 64>(a, plan, stream)
+           : plan.threads == 128 ? launch_distill<T, 128>(a, plan, stream)
+                                 : launch_distill<T, 256>(a, plan, stream);
 }
 
 int distill_timeout_take(int *out)

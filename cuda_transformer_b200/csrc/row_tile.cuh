@@ -28,10 +28,10 @@ struct RowPlan
     int smem;               // dynamic shared memory of a block
 };
 
-// Cluster and block size for rows of `cols` elements of `size` bytes, with more(plan) bytes of shared memory
+// Cluster and block size (least .. most threads) for rows of `cols` elements of `size` bytes, with more(plan) bytes of shared memory
 // besides the segment. B200AMP_ERR_LIMIT where a row does not fit the largest cluster.
 template <typename More>
-int plan_rows(long long rows, int cols, int size, More more, RowPlan *plan)
+int plan_rows(long long rows, int cols, int size, int least, int most, More more, RowPlan *plan)
 {
     const int sms = sm_count();
     if (sms <= 0)
@@ -65,10 +65,19 @@ int plan_rows(long long rows, int cols, int size, More more, RowPlan *plan)
         cluster *= 2;
         fill(cluster, 256);
     }
-    // Short segments: more and smaller blocks (4096 rows of 4160 fp16 columns, distill_loss: 128 threads 62 us, 256 threads 102 us).
-    if (plan->segment * size <= 20 * 1024)
+    // A row costs a block some thousand cycles of barriers and short chains whatever its length, so short segments want
+    // more and smaller blocks side by side (distill_loss, 8192 rows: of 700 fp16 columns 64 threads 59 us, 128 threads
+    // 86 us, 256 threads 158 us; of 12,000 bf16 columns 117, 126 and 170 us), unless there are hardly rows for them; and
+    // a block that has an SM to itself wants its threads (top_logits, 510 rows of 128,001 bf16 columns: 256 threads
+    // 160 us, 512 threads 121 us).
+    if (rows * cluster > 2ll * sms)
     {
-        fill(cluster, 128);
+        const int bytes = plan->segment * size;
+        fill(cluster, bytes <= 32 * 1024 ? least : bytes <= 56 * 1024 ? 128 : 256);
+    }
+    if (plan->smem > 112 * 1024)
+    {
+        fill(cluster, most);
     }
     if (plan->smem > MAX_ROW_SMEM)
     {

@@ -613,7 +613,7 @@ static int launch_top(TopArgs a, cudaStream_t stream)
     }
     RowPlan plan;
     const int rc = plan_rows(
-        a.rows, a.vocab, sizeof(T), [&](const RowPlan &p) {
+        a.rows, a.vocab, sizeof(T), 128, 512, [&](const RowPlan &p) {
             return (a.room + a.room / 2 + 2 * a.k + (p.cluster > 1 && p.cluster * a.k <= MOST_BROUGHT ? p.cluster * a.k : 0)) *
                    static_cast<int>(sizeof(unsigned long long));
         },
@@ -622,8 +622,9 @@ static int launch_top(TopArgs a, cudaStream_t stream)
     {
         return rc;
     }
-    return plan.threads == 128 ? launch_rows(top_rows_kernel<T, 128>, a, plan, 128, a.rows, stream)
-                               : launch_rows(top_rows_kernel<T, 256>, a, plan, 256, a.rows, stream);
+    return plan.threads == 128   ? launch_rows(top_rows_kernel<T, 128>, a, plan, 128, a.rows, stream)
+           : plan.threads == 256 ? launch_rows(top_rows_kernel<T, 256>, a, plan, 256, a.rows, stream)
+                                 : launch_rows(top_rows_kernel<T, 512>, a, plan, 512, a.rows, stream);
 }
 
 int top_timeout_take(int *out)

@@ -381,6 +381,32 @@ def test_distill_many_rows_same_bits_every_time_and_any_loss_scale():
     assert torch.equal(a["dlogits"] * 4, c["dlogits"]) and a["loss"] == c["loss"]
 
 
+@pytest.mark.parametrize("rows,vocab,dtype,k,T,rest,hard", [
+    (331, 4098, "f16", 16, 1.0, True, 0.5), (331, 12000, "f32", 8, 2.0, False, 0.3), (305, 12001, "f32", 8, 1.0, True, 0.0),
+    (301, 30011, "bf16", 70, 1.0, True, 0.5), (299, 50257, "f16", 33, 1.0, False, 0.0), (640, 9, "f16", 3, 1.0, True, 0.5),
+    (700, 130, "bf16", 130, 0.8, True, 0.2)])
+def test_distill_more_rows_than_blocks(rows, vocab, dtype, k, T, rest, hard):
+    """Every size of block, each with several rows one behind the other, some of which do not count."""
+    p = _problem(rows, vocab, vocab + 2, TYPES[dtype], k, T, rest, hard, ignored=0.3)
+    p["targets"][:40] = -1                                      # whole blocks begin with rows that do not count
+    p["indices"][rows - 1, 1:] = p["indices"][rows - 1, 0]
+    _check(p, _run(p))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,k", [(331, 4098, "f16", 16), (303, 20011, "bf16", 100), (299, 50257, "f16", 64),
+                                                (160, 100003, "f16", 300), (900, 33, "f32", 33), (40, 131072, "f32", 1024)])
+def test_top_logits_more_rows_than_blocks(rows, vocab, dtype, k):
+    z = (torch.randn(rows, vocab, generator=torch.Generator().manual_seed(rows + k)) * 2).to(TYPES[dtype])
+    z[::5, ::7] = 1.0                                           # many ties
+    z[3] = -math.inf
+    values, indices, lse = _top(z, k, vocab)
+    want = torch.sort(z.float(), dim=1, descending=True, stable=True)
+    assert torch.equal(indices.long(), want.indices[:, :k]) and torch.equal(values.float(), want.values[:, :k])
+    exact = torch.logsumexp(z.double(), dim=1)
+    same = lse.double() == exact
+    assert bool((same | ((lse.double() - exact).abs() <= _rel(vocab, 30.0) + 2 * U * exact.abs())).all())
+
+
 def test_distill_overflow_becomes_inf():
     """A loss scale that takes the gradient out of fp16's range: inf in the gradient, so that the step is skipped."""
     p = _problem(1, 64, 64, torch.float16, 2, 1.0, False, 1.0)

@@ -885,6 +885,10 @@ extern "C" B200AMP_API int b200amp_distill_loss(const void *logits, long long ld
     {
         k = 0;
     }
+    if (k == 0)
+    {
+        lse = nullptr;                          // no teacher: not read
+    }
     if (k > 0 && rows > 0)
     {
         B200AMP_REQUIRE(values != nullptr && indices != nullptr, "distill_loss: k = %d needs values and indices", k);

@@ -18,6 +18,7 @@ Two layers:
   the passes (peer loads and stores over NVLink, or the copy engines) and orders the
   ranks with the library's own bounded flag words. HostGradientFeed (mixed into the
   owners) feeds steps from pinned host memory through two gradient arenas taking turns.
+  LossCalls (losses.py, mixed in too) gives them the losses that open the backward pass.
 
 torch is used for device memory, streams and the process group only; every
 arithmetic step runs in the CUDA kernels of the library.

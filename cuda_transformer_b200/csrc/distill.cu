@@ -305,6 +305,11 @@ __device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, 
 //     summed    (the cluster's) every warp's sums are with every block
 //     factors   the row's factors are known
 //     written   the gradient is out; the row's place may be filled again
+// 8192 rows of 50257 fp16 columns (k 64, rest and label) take 350 us, 1.6 GB, 4.6 TB/s; the powers alone would take 181 us
+// of the special function unit, the bytes 246 us. A block's rows are behind one another, so what bounds it is a row's
+// chain: at two blocks an SM about 20,000 cycles, 6,500 for the sums, 5,500 for the gradient, the rest barriers, the
+// record and the factors. Registers for two blocks of 256 threads an SM (or eight of 64): with fewer, spills go past
+// the little L1 that the rows leave (422 us).
 template <typename T, int SWEEP>
 __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(const DistillArgs a, const RowPlan plan)
 {

@@ -41,31 +41,31 @@ def loss_workspace(device="cuda") -> torch.Tensor:
 
 
 def _matrix(t: torch.Tensor, name: str, device: int = -1):
-    """(pointer, row stride in elements, rows, columns, type code) of a 2-D CUDA tensor."""
-    code = _DTYPES.get(t.dtype)
-    if t.dim() != 2 or not t.is_cuda or code is None:
+    """(pointer, row stride in elements, rows, columns, type code, device) of a 2-D CUDA tensor."""
+    code, on = _DTYPES.get(t.dtype), t.get_device()     # -1: not on a GPU
+    if t.dim() != 2 or on < 0 or code is None:
         raise ValueError(f"{name}: expected a 2-D CUDA tensor of fp16, bf16 or fp32, got {t.dim()}-D {t.dtype} on {t.device}")
-    if device >= 0 and t.get_device() != device:
+    if device >= 0 and on != device:
         raise ValueError(f"{name} is on {t.device}, expected cuda:{device}")
     rows, cols = t.shape
     ld, step = t.stride()
     if step != 1 and cols > 1:
         raise ValueError(f"{name}: the columns of a row must be next to each other (strides {t.stride()})")
-    return t.data_ptr(), (ld if rows > 1 else cols), rows, cols, code
+    return t.data_ptr(), (ld if rows > 1 else cols), rows, cols, code, on
 
 
 def _array(t: Optional[torch.Tensor], name: str, dtype, shape, device: int) -> Optional[int]:
     """Pointer of a contiguous tensor of this type and shape, or None for None."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != shape or not t.is_cuda or t.get_device() != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on cuda:{device}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _bytes(t: torch.Tensor, name: str, least: int, device: int) -> int:
-    if not t.is_cuda or t.get_device() != device or not t.is_contiguous() or t.nbytes < least:
+    if t.get_device() != device or not t.is_contiguous() or t.nbytes < least:
         raise ValueError(f"{name}: expected a contiguous tensor of {least} bytes or more on cuda:{device}")
     return t.data_ptr()
 
@@ -91,8 +91,7 @@ def top_logits(logits: torch.Tensor, k: int, values: torch.Tensor, indices: torc
     """The k largest of every row's first `vocab` columns (default: all of them) into values[rows, k] (the
     logits' type) and indices[rows, k] (int32), in descending order, ties to the lowest column; and, if lse is
     given, log sum exp(z / temperature) over the row into lse[rows] (fp32)."""
-    ptr, ld, rows, cols, dtype = _matrix(logits, "logits")
-    dev = logits.get_device()
+    ptr, ld, rows, cols, dtype, dev = _matrix(logits, "logits")
     vocab = cols if vocab is None else vocab
     if not 1 <= vocab <= cols:
         raise ValueError(f"vocab = {vocab}: the logits have {cols} columns")
@@ -110,12 +109,11 @@ def distill_loss(logits: torch.Tensor, dlogits: Optional[torch.Tensor], targets:
     state's loss scale. values / indices [rows, k] are the teacher's listed logits (index < 0: empty slot), lse
     its log-sum-exp at the same temperature, or None to normalise over the listed logits alone. Columns from
     `vocab` on pad the vocabulary. dlogits may be logits itself. Without a teacher pass None for the three."""
-    ptr, ld, rows, cols, dtype = _matrix(logits, "logits")
-    dev = logits.get_device()
+    ptr, ld, rows, cols, dtype, dev = _matrix(logits, "logits")
     vocab = cols if vocab is None else vocab
     dptr, dld = None, cols
     if dlogits is not None:
-        dptr, dld, drows, dcols, ddtype = _matrix(dlogits, "dlogits", dev)
+        dptr, dld, drows, dcols, ddtype, _ = _matrix(dlogits, "dlogits", dev)
         if drows != rows or dcols != cols or ddtype != dtype:
             raise ValueError(f"dlogits: expected {logits.dtype} {tuple(logits.shape)}, got {dlogits.dtype} {tuple(dlogits.shape)}")
     k, vtype = 0, dtype
@@ -142,11 +140,10 @@ def balance_loss(logits: torch.Tensor, dlogits: Optional[torch.Tensor], chosen: 
     targets >= 0 (None: all): loss[1], the choices of each expert into counts[experts] (int32), and (dlogits not
     None) the gradient times the state's loss scale, added to dlogits if accumulate. chosen[rows, k] (int32) are
     the router's choices, negative where one was not made. add_to_state adds the loss to state.loss."""
-    ptr, ld, rows, experts, dtype = _matrix(logits, "logits")
-    dev = logits.get_device()
+    ptr, ld, rows, experts, dtype, dev = _matrix(logits, "logits")
     dptr, dld = None, experts
     if dlogits is not None:
-        dptr, dld, drows, dcols, ddtype = _matrix(dlogits, "dlogits", dev)
+        dptr, dld, drows, dcols, ddtype, _ = _matrix(dlogits, "dlogits", dev)
         if drows != rows or dcols != experts or ddtype != dtype:
             raise ValueError(f"dlogits: expected {logits.dtype} {tuple(logits.shape)}, got {dlogits.dtype} {tuple(dlogits.shape)}")
     if chosen.dim() != 2:

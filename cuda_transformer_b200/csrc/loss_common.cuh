@@ -130,26 +130,6 @@ __device__ __forceinline__ double block_sum_f64(double v, double *scratch)
     return total;
 }
 
-template <int THREADS>
-__device__ __forceinline__ float block_max_nan(float v, double *scratch)
-{
-    float *s = reinterpret_cast<float *>(scratch);
-    v = warp_max_nan(v);
-    if ((threadIdx.x & 31) == 0)
-    {
-        s[threadIdx.x >> 5] = v;
-    }
-    __syncthreads();
-    float best = s[0];
-#pragma unroll
-    for (int w = 1; w < THREADS / 32; w++)
-    {
-        best = max_nan(best, s[w]);
-    }
-    __syncthreads();
-    return best;
-}
-
 // True (in every thread) for the block that takes the last ticket of `blocks`: all that the other
 // blocks wrote before theirs is visible to it. The ticket is reset for the next launch.
 __device__ __forceinline__ bool take_last_ticket(unsigned int *ticket, unsigned int blocks, int *shared_flag)

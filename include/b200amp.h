@@ -483,7 +483,8 @@ B200AMP_API int b200amp_distill_loss(const void *logits, long long ld, void *dlo
  * (rows that do not count: 0), or, with accumulate != 0, is added to what dlogits holds (rows that do not
  * count: left as they are). add_to_state != 0 also adds the loss to st->loss (st->n_valid is not
  * touched), for a loss that joins the model's: call it after the one that writes st->loss. n == 0: loss 0.
- * An expert beyond the last is not counted and makes the loss and every gradient NaN. dlogits may be null
+ * An expert beyond the last is not counted and makes the loss and every gradient NaN. NaN, +inf or nothing
+ * but -inf in a row that counts makes the loss and that row's gradient NaN. dlogits may be null
  * (the counts and the loss alone) or the logits themselves (accumulate == 0, same ld).
  * rows >= 0, 1 <= experts <= 1024, experts <= ld and dld, 1 <= k <= 1024, rows * k < 2^31. At most two
  * launches. No reference counterpart (its models have no experts). */

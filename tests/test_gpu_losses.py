@@ -603,6 +603,20 @@ def test_balance_an_expert_beyond_the_last_and_masked_logits():
     assert math.isfinite(got["loss"]) and bool(torch.isfinite(got["dlogits"]).all())
 
 
+@pytest.mark.parametrize("rows,experts", [(40, 8), (700, 64), (300, 67)])
+def test_balance_a_row_without_a_softmax_is_nan_alone(rows, experts):
+    z, chosen, targets = _balance_problem(rows, experts, torch.float16, 8)
+    bad = {3: -math.inf, 11: math.nan, 20: math.inf}
+    for row, value in bad.items():
+        z[row, :] = value if value == -math.inf else z[row]
+        z[row, experts - 1] = value
+    got = _balance(z, chosen, None)
+    assert math.isnan(got["loss"]) and torch.equal(got["counts"], R.balance(z, chosen, None, 0.01, 1.0)["counts"])
+    assert torch.isnan(got["dlogits"].float()).any(1).nonzero()[:, 0].tolist() == list(bad)
+    targets[list(bad)] = -1                                     # the same rows, left out
+    _check_balance(z.nan_to_num(0.0, 0.0, 0.0), chosen, targets, _balance(z, chosen, targets))
+
+
 # ---------------------------------------------------------------- streams, graphs, the step
 
 def test_calls_on_two_streams_with_a_workspace_each():

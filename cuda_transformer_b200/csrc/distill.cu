@@ -437,13 +437,15 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
         cluster.sync();                         // every block of the cluster runs before one writes to another
     }
 
-    // The first trip has no row yet (row < 0): it starts the first copy and reads the first record.
+    // The first trip has no row yet (row < 0): it starts the first copy and reads the first record. The rows that count
+    // take the two places of the sums and of the records in turn: between two uses of a place there is then always one
+    // row whose barriers all readers of the first use have reached (a row that does not count has no barrier).
     bool twice = false;
     unsigned int phase = 0;                     // of row_bar
     float soft_scale = 0.0f, hard_scale = 0.0f;
     long long n_valid = 0;
     int y = -1, parity = 0;
-    for (long long row = blockIdx.x / blocks - clusters; row < a.rows; row += clusters, parity ^= 1)
+    for (long long row = blockIdx.x / blocks - clusters; row < a.rows; row += clusters)
     {
         T *out = a.dlogits != nullptr && row >= 0 ? static_cast<T *>(a.dlogits) + row * a.dld : nullptr;
         const int next_y = label_of(row + clusters);
@@ -797,6 +799,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
             }
         }
         y = next_y;
+        parity ^= next_y >= 0 ? 1 : 0;
     }
 
     if (!take_last_ticket(&a.ws->distill_ticket, gridDim.x, &last_block))

@@ -310,7 +310,7 @@ def pass2_ag_f16_ce(master, m, v, reduced16, weights16_by_rank: Sequence[int], m
 
 def device_error() -> int:
     """Bit mask of what gave up a bounded wait on the current device since the last call (1: a bulk
-    copy of the staged pass 2, 2: a wait on another rank); reading clears it. Synchronises."""
+    copy of the staged pass 2, 2: a wait on another rank, 4: a loss's copy of a row); reading clears it. Synchronises."""
     out = C.c_int()
     check(_lib.load().b200amp_device_error(C.byref(out)))
     return out.value

@@ -3,6 +3,7 @@
 // helpers (capture / launch, cuda/graph.cu:17-41 of the reference).
 
 #include <atomic>
+#include <climits>
 #include <cstring>
 #include <new>
 
@@ -67,7 +68,7 @@ int sm_count()
 
 Tunables &tunables()
 {
-    static Tunables t = {4, 2, 1, 256, 0, 6, 0, 8, 0, 16, 2};   // measured best on B200 at the 1.3 B arena
+    static Tunables t = {4, 2, 1, 256, 0, 6, 0, 8, 0, 16, 2, 0};   // measured best on B200 at the 1.3 B arena
     return t;
 }
 
@@ -90,6 +91,7 @@ static const Knob KNOBS[] = {
     {"ag_blocks_per_sm", &Tunables::ag_blocks_per_sm, 0, 32},
     {"bridge_blocks_per_sm", &Tunables::bridge_blocks_per_sm, 1, 32},
     {"ce_lanes", &Tunables::ce_lanes, 1, 7},
+    {"loss_test_starve", &Tunables::loss_test_starve, 0, INT_MAX},
 };
 
 } // namespace b200amp

@@ -32,6 +32,7 @@ struct DistillArgs
     b200amp_step_state *st;
     float *row_loss;
     LossWorkspace *ws;
+    long long starved;      // row whose copy a test keeps from completing, -1: none
 };
 
 // Rows that count: every block counts for itself, as the gradient needs the number from its first row on.
@@ -322,6 +323,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
     __shared__ int label_listed[2], beyond_listed[2];
     __shared__ uint64_t row_bar;
     __shared__ int last_block;
+    __shared__ unsigned int lost;               // a copy of this block's never came (1 + its phase): its rows from there on are NaN
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool sweeps = warp < WARPS;
     const cg::cluster_group cluster = cg::this_cluster();
@@ -429,6 +431,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
     }
     if (tid == 0)
     {
+        lost = 0u;
         row_barrier_init(&row_bar);
     }
     __syncthreads();
@@ -462,9 +465,9 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
         {
             if (sweeps)
             {
-                if (!row_wait(&row_bar, phase))
+                if (lost == 0u && !row_wait(&row_bar, phase))
                 {
-                    beyond_listed[parity] = 1;  // the row is NaN
+                    lost = 1u + phase;
                     g_row_timeout = 1;
                 }
                 phase ^= 1u;
@@ -588,9 +591,9 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                     part = warp_sum_f64(part);
                     own = warp_sum_f64(own);
                 }
-                if (beyond_listed[parity] != 0)
+                if (beyond_listed[parity] != 0 || lost != 0u)
                 {
-                    own = nan("");              // a column beyond the vocabulary: the row is NaN
+                    own = nan("");              // a column beyond the vocabulary, or no row: the row is NaN
                 }
                 if (lane < blocks)
                 {
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                 const float o_in_all = shifted_fast(m_o, m, c_t);
                 const float total = fmaf(others, o_in_all, listed_t);
                 const double rest = a.lse != nullptr && a.k > 0 && others > 0.0f ? fmax(0.0, 1.0 - mass) : 0.0;
-                poison = !isfinite(m) || (hard && !label_in) ? NAN : 0.0f;
+                poison = !isfinite(m) || (hard && !label_in) || own != own ? NAN : 0.0f;
                 const float whole = static_cast<float>(mass + rest) + poison;
                 const float u_in_all_1 = two ? shifted_fast(all_u, m, c_1) : u_in_o * o_in_all;
                 not_y_1 = fmaf(u_1, u_in_all_1, listed_1);                      // all but the label, where that is not listed
@@ -762,7 +765,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
         if (sweeps && next_y >= 0)
         {
             tile.start(static_cast<const T *>(a.logits) + (row + clusters) * a.ld, first, plan.segment, a.vocab, a.cols,
-                       &row_bar);
+                       &row_bar, lost == 0u, row + clusters == a.starved && rank == blocks - 1 ? 16u : 0u);
             if (a.k > 0)
             {
                 if (y < 0)
@@ -800,6 +803,10 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
         }
         y = next_y;
         parity ^= next_y >= 0 ? 1 : 0;
+    }
+    if (tid == 0 && lost != 0u)
+    {
+        row_wait(&row_bar, lost - 1u);          // shared memory is not handed back with a copy on its way
     }
 
     if (!take_last_ticket(&a.ws->distill_ticket, gridDim.x, &last_block))
@@ -909,7 +916,8 @@ extern "C" B200AMP_API int b200amp_distill_loss(const void *logits, long long ld
     B200AMP_REQUIRE(aligned(st, 4) && aligned(row_loss, 4) && aligned(workspace, 16),
                     "distill_loss: state, row_loss or workspace is misaligned");
     DistillArgs a = {logits, dlogits, ld, dld, rows, vocab, cols, targets, values, indices, lse, value_dtype, k,
-                     temperature, soft_weight, hard_weight, st, row_loss, static_cast<LossWorkspace *>(workspace)};
+                     temperature, soft_weight, hard_weight, st, row_loss, static_cast<LossWorkspace *>(workspace),
+                     tunables().loss_test_starve - 1ll};
     switch (dtype)
     {
     case B200AMP_F16:

@@ -37,6 +37,7 @@ struct Tunables
     int ag_blocks_per_sm;       // resident CTAs per SM of the fused pass 2 + all-gather, 0 = by rank count
     int bridge_blocks_per_sm;   // CTAs per SM asked for by the fp32 -> fp16 bridge (cast + pass 1)
     int ce_lanes;               // copy streams the copy-engine forms of the ZeRO-1 step spread their copies over
+    int loss_test_starve;       // test hook of the losses: r makes the copy of row r - 1 never complete, 0: none (see row_tile.cuh)
 };
 Tunables &tunables();
 

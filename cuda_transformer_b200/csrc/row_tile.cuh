@@ -238,9 +238,13 @@ __device__ __forceinline__ void row_barrier_init(uint64_t *bar)
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" : : "r"(shared_address(bar)) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" : : : "memory");
 }
-__device__ __forceinline__ void row_copy(void *dst, const void *src, unsigned bytes, uint64_t *bar)
+// never: bytes that are announced and do not come (a test's, else 0).
+__device__ __forceinline__ void row_copy(void *dst, const void *src, unsigned bytes, unsigned never, uint64_t *bar)
 {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" : : "r"(shared_address(bar)), "r"(bytes) : "memory");
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                 :
+                 : "r"(shared_address(bar)), "r"(bytes + never)
+                 : "memory");
     if (bytes > 0)
     {
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -249,10 +253,13 @@ __device__ __forceinline__ void row_copy(void *dst, const void *src, unsigned by
                      : "memory");
     }
 }
-// Bounded: false when the limit ran out (about a second), which only a copy that never completes can bring about.
+// Bounded: false when the limit ran out, which only a copy that never completes can bring about. A poll of an open phase
+// takes 2 us (distill_loss) to 4 us (top_logits), as the hardware suspends the thread: half a second to one second in all. The
+// block then starts no copy any more (the barrier's phase is still open), gives the one in flight another such wait
+// before it leaves, and marks this row and those behind it.
 __device__ __forceinline__ bool row_wait(uint64_t *bar, unsigned parity)
 {
-    for (unsigned tries = 0; tries < 1u << 22; tries++)
+    for (unsigned tries = 0; tries < 1u << 18; tries++)
     {
         unsigned ok;
         asm volatile("{\n\t.reg .pred p;\n\t"
@@ -303,7 +310,9 @@ struct RowTile
 
     // Starts the copy of columns [first, first + valid) of the row at z; padding and ends are set to -inf. Every
     // thread, after a barrier behind the last use of the segment; the row is there after row_wait and a barrier.
-    __device__ __forceinline__ void start(const T *z, int first_column, int segment, int vocab, int cols, uint64_t *bar)
+    // copy: false in a block whose earlier copy never came.
+    __device__ __forceinline__ void start(const T *z, int first_column, int segment, int vocab, int cols, uint64_t *bar, bool copy,
+                                          unsigned never)
     {
         first = first_column;
         valid = max(0, min(segment, vocab - first));
@@ -314,9 +323,9 @@ struct RowTile
         vecs = held > 0 ? (lead + held + N - 1) / N : 0;
         const int whole_first = lead > 0 ? 1 : 0, whole_end = (lead + valid) / N;      // vectors inside the columns
         src -= skew;
-        if (threadIdx.x == 0)
+        if (threadIdx.x == 0 && copy)
         {
-            row_copy(buf + 16 * whole_first, src + 16 * whole_first, 16u * max(0, whole_end - whole_first), bar);
+            row_copy(buf + 16 * whole_first, src + 16 * whole_first, 16u * max(0, whole_end - whole_first), never, bar);
         }
         // the elements of the other vectors: at most N - 1 at the front, then the end and the padding. Those that hold
         // logits (2 N - 2 at most, one a thread) are fetched here and put in place by finish.

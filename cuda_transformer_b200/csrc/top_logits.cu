@@ -23,6 +23,7 @@ struct TopArgs
     void *values;
     int *indices;
     float *lse;
+    long long starved;          // row whose copy a test keeps from completing, -1: none
 };
 
 // A key that orders as the numbers do: -0 as +0, every NaN above +inf.
@@ -193,6 +194,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     __shared__ float warp_m[WARPS], warp_s[WARPS];
     __shared__ float2 block_ms[2];              // of two rows: this segment's maximum and sum
     __shared__ int collected, met;              // columns that reach, vectors that hold some
+    __shared__ unsigned int lost;               // a copy of this block's never came (1 + its phase): its rows from there on are not looked at
+    __shared__ int failed[2];                   // of two rows: some block of the cluster has not got its segment
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const cg::cluster_group cluster = cg::this_cluster();
     const int blocks = plan.cluster, rank = blocks > 1 ? static_cast<int>(cluster.block_rank()) : 0;
@@ -212,10 +215,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     unsigned long long *const others = best0 + 2 * a.k;     // every segment's, brought over where they are few
     const bool brought = blocks * a.k <= MOST_BROUGHT;
     auto start = [&](long long row) {
-        tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.vocab, &row_bar);
+        tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.vocab, &row_bar, lost == 0u,
+                   row == a.starved && rank == blocks - 1 ? 16u : 0u);
     };
     if (tid == 0)
     {
+        lost = 0u;
+        failed[0] = failed[1] = 0;
         row_barrier_init(&row_bar);
     }
     __syncthreads();
@@ -234,21 +240,29 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     for (; row < a.rows; row += clusters, parity ^= 1)
     {
         unsigned long long *const best = best0 + parity * a.k;
-        const int valid = tile.valid;
-        const int kept = min(a.k, valid);       // of this segment
         if (tid == 0)
         {
             collected = 0;
             met = 0;
         }
-        const bool there = row_wait(&row_bar, phase);
-        phase ^= 1u;
-        tile.finish();
-        if (!there)
+        if (lost == 0u && !row_wait(&row_bar, phase))
         {
+            lost = 1u + phase;
             g_row_timeout = 1;
         }
+        phase ^= 1u;
+        tile.finish();
         __syncthreads();
+        if (lost != 0u)
+        {
+            tile.valid = tile.vecs = 0;
+            if (tid < blocks)
+            {
+                (blocks > 1 ? cluster.map_shared_rank(failed, tid) : failed)[parity] = 1;
+            }
+        }
+        const int valid = tile.valid;
+        const int kept = min(a.k, valid);       // of this segment
 
         // maxima of the groups
         Vec16<T> group;
@@ -544,7 +558,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
             }
             __syncthreads();
         }
-        for (int j = tid; j < kept; j += THREADS)
+        const bool none = failed[parity] != 0;
+        for (int j = tid; j < kept && !none; j += THREADS)
         {
             const unsigned long long entry = best[j];
             int place = j;
@@ -577,10 +592,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
         }
         if (rank == 0)
         {
-            for (int j = a.vocab + tid; j < a.k; j += THREADS)
+            for (int j = tid + (none ? 0 : a.vocab); j < a.k; j += THREADS)
             {
-                a.indices[row * a.k + j] = -1;  // fewer columns than asked for
-                static_cast<T *>(a.values)[row * a.k + j] = minus_infinity<T>();
+                a.indices[row * a.k + j] = -1;  // fewer columns than asked for, or no row
+                static_cast<T *>(a.values)[row * a.k + j] = from_float<T>(none ? NAN : -INFINITY);
             }
             if (sums && tid == 0)
             {
@@ -596,9 +611,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
                     total += ms.x == -INFINITY ? 0.0 : ms.y * exp((static_cast<double>(ms.x) - all) * inv_t);
                 }
                 // a row of nothing but -inf has the log of 0; +inf has itself
-                a.lse[row] = isinf(all) ? all : static_cast<float>(all * inv_t + log(total)) + (there ? 0.0f : NAN);
+                a.lse[row] = isinf(all) ? all : static_cast<float>(all * inv_t + log(total));
+                if (none)
+                {
+                    a.lse[row] = NAN;
+                }
             }
         }
+    }
+    if (tid == 0 && lost != 0u)
+    {
+        row_wait(&row_bar, lost - 1u);          // shared memory is not handed back with a copy on its way
     }
     if (blocks > 1)
     {
@@ -659,7 +682,7 @@ extern "C" B200AMP_API int b200amp_top_logits(const void *logits, int dtype, lon
     {
         return B200AMP_OK;
     }
-    const TopArgs a = {logits, ld, rows, vocab, k, 0, temperature, values, indices, lse};
+    const TopArgs a = {logits, ld, rows, vocab, k, 0, temperature, values, indices, lse, tunables().loss_test_starve - 1ll};
     switch (dtype)
     {
     case B200AMP_F16:

@@ -323,7 +323,6 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
     __shared__ int label_listed[2], beyond_listed[2];
     __shared__ uint64_t row_bar;
     __shared__ int last_block;
-    __shared__ unsigned int lost;               // a copy of this block's never came (1 + its phase): its rows from there on are NaN
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool sweeps = warp < WARPS;
     const cg::cluster_group cluster = cg::this_cluster();
@@ -431,7 +430,6 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
     }
     if (tid == 0)
     {
-        lost = 0u;
         row_barrier_init(&row_bar);
     }
     __syncthreads();
@@ -444,7 +442,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
     // take the two places of the sums and of the records in turn: between two uses of a place there is then always one
     // row whose barriers all readers of the first use have reached (a row that does not count has no barrier).
     bool twice = false;
-    unsigned int phase = 0;                     // of row_bar
+    unsigned int phase = 0u;                    // of row_bar, with what RowTile::wait adds
     float soft_scale = 0.0f, hard_scale = 0.0f;
     long long n_valid = 0;
     int y = -1, parity = 0;
@@ -465,13 +463,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
         {
             if (sweeps)
             {
-                if (lost == 0u && !row_wait(&row_bar, phase))
-                {
-                    lost = 1u + phase;
-                    g_row_timeout = 1;
-                }
-                phase ^= 1u;
-                tile.finish();
+                tile.wait(&row_bar, phase);
             }
             if (__syncthreads_or(twice))        // arrived
             {
@@ -591,9 +583,9 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                     part = warp_sum_f64(part);
                     own = warp_sum_f64(own);
                 }
-                if (beyond_listed[parity] != 0 || lost != 0u)
+                if (beyond_listed[parity] != 0)
                 {
-                    own = nan("");              // a column beyond the vocabulary, or no row: the row is NaN
+                    own = nan("");              // a column beyond the vocabulary: the row is NaN
                 }
                 if (lane < blocks)
                 {
@@ -673,7 +665,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                 const float o_in_all = shifted_fast(m_o, m, c_t);
                 const float total = fmaf(others, o_in_all, listed_t);
                 const double rest = a.lse != nullptr && a.k > 0 && others > 0.0f ? fmax(0.0, 1.0 - mass) : 0.0;
-                poison = !isfinite(m) || (hard && !label_in) || own != own ? NAN : 0.0f;
+                poison = !isfinite(m) || (hard && !label_in) ? NAN : 0.0f;
                 const float whole = static_cast<float>(mass + rest) + poison;
                 const float u_in_all_1 = two ? shifted_fast(all_u, m, c_1) : u_in_o * o_in_all;
                 not_y_1 = fmaf(u_1, u_in_all_1, listed_1);                      // all but the label, where that is not listed
@@ -765,7 +757,7 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
         if (sweeps && next_y >= 0)
         {
             tile.start(static_cast<const T *>(a.logits) + (row + clusters) * a.ld, first, plan.segment, a.vocab, a.cols,
-                       &row_bar, lost == 0u, row + clusters == a.starved && rank == blocks - 1 ? 16u : 0u);
+                       &row_bar, phase, row + clusters == a.starved && rank == blocks - 1);
             if (a.k > 0)
             {
                 if (y < 0)
@@ -804,9 +796,9 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
         y = next_y;
         parity ^= next_y >= 0 ? 1 : 0;
     }
-    if (tid == 0 && lost != 0u)
+    if (tid == 0)
     {
-        row_wait(&row_bar, lost - 1u);          // shared memory is not handed back with a copy on its way
+        row_leave(&row_bar, phase);
     }
 
     if (!take_last_ticket(&a.ws->distill_ticket, gridDim.x, &last_block))

@@ -254,9 +254,7 @@ __device__ __forceinline__ void row_copy(void *dst, const void *src, unsigned by
     }
 }
 // Bounded: false when the limit ran out, which only a copy that never completes can bring about. A poll of an open phase
-// takes 2 us (distill_loss) to 4 us (top_logits), as the hardware suspends the thread: half a second to one second in all. The
-// block then starts no copy any more (the barrier's phase is still open), gives the one in flight another such wait
-// before it leaves, and marks this row and those behind it.
+// takes 2 us (distill_loss) to 4 us (top_logits), as the hardware suspends the thread: half a second to one second in all.
 __device__ __forceinline__ bool row_wait(uint64_t *bar, unsigned parity)
 {
     for (unsigned tries = 0; tries < 1u << 18; tries++)
@@ -279,6 +277,16 @@ __device__ __forceinline__ bool row_wait(uint64_t *bar, unsigned parity)
 __device__ __forceinline__ void before_copies()
 {
     asm volatile("fence.proxy.async.shared::cta;" : : : "memory");
+}
+
+// NaN in the place of a row that did not come. A call, so that it costs the rows that come nothing.
+static __device__ __noinline__ void lose_row(char *buf, int vecs, int threads)
+{
+    g_row_timeout = 1;
+    for (int i = threadIdx.x; i < vecs; i += threads)
+    {
+        reinterpret_cast<uint4 *>(buf)[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+    }
 }
 
 // This block's segment of the current row.
@@ -310,9 +318,9 @@ struct RowTile
 
     // Starts the copy of columns [first, first + valid) of the row at z; padding and ends are set to -inf. Every
     // thread, after a barrier behind the last use of the segment; the row is there after row_wait and a barrier.
-    // copy: false in a block whose earlier copy never came.
-    __device__ __forceinline__ void start(const T *z, int first_column, int segment, int vocab, int cols, uint64_t *bar, bool copy,
-                                          unsigned never)
+    // phase: the one that wait() keeps. starved: a test's, this copy never completes.
+    __device__ __forceinline__ void start(const T *z, int first_column, int segment, int vocab, int cols, uint64_t *bar, unsigned phase,
+                                          bool starved)
     {
         first = first_column;
         valid = max(0, min(segment, vocab - first));
@@ -323,9 +331,9 @@ struct RowTile
         vecs = held > 0 ? (lead + held + N - 1) / N : 0;
         const int whole_first = lead > 0 ? 1 : 0, whole_end = (lead + valid) / N;      // vectors inside the columns
         src -= skew;
-        if (threadIdx.x == 0 && copy)
+        if (threadIdx.x == 0 && phase < 2u)
         {
-            row_copy(buf + 16 * whole_first, src + 16 * whole_first, 16u * max(0, whole_end - whole_first), never, bar);
+            row_copy(buf + 16 * whole_first, src + 16 * whole_first, 16u * max(0, whole_end - whole_first), starved ? 16u : 0u, bar);
         }
         // the elements of the other vectors: at most N - 1 at the front, then the end and the padding. Those that hold
         // logits (2 N - 2 at most, one a thread) are fetched here and put in place by finish.
@@ -353,9 +361,20 @@ struct RowTile
             before_copies();
         }
     }
-    // Before the barrier behind row_wait: the elements that the copy engine does not move.
-    __device__ __forceinline__ void finish()
+    // Waits for the row and puts the elements in place that the copy engine does not move; a barrier follows. phase: the
+    // barrier's, 0 at first. Where the wait gives up, 2 is added to it and stays: the phase is still open, so this block
+    // waits for and (thread 0) starts no copy any more, and from this row on it has NaN in place of the logits.
+    __device__ __forceinline__ void wait(uint64_t *bar, unsigned &phase)
     {
+        if (phase < 2u && row_wait(bar, phase))
+        {
+            phase ^= 1u;
+        }
+        else
+        {
+            phase |= 2u;
+            lose_row(buf, vecs, THREADS);
+        }
         if (edge_at >= 0)
         {
             reinterpret_cast<T *>(buf)[edge_at] = edge;
@@ -366,6 +385,16 @@ struct RowTile
         }
     }
 };
+
+// Before a block leaves, thread 0: another bounded wait for a copy that was given up, so that shared memory is not handed
+// back with it on its way.
+__device__ __forceinline__ void row_leave(uint64_t *bar, unsigned phase)
+{
+    if (phase >= 2u)
+    {
+        row_wait(bar, phase & 1u);
+    }
+}
 
 // *out |= 1 if a wait for a row's copy gave up in this source file's kernels since the last call (clears it).
 static int take_row_timeout(int *out)

@@ -99,7 +99,7 @@ __device__ __forceinline__ void sort_entries(unsigned long long *list, int n, in
 // The `kept` largest columns of the segment into list, in no order: their smallest key by four rounds of a histogram
 // (8 bits a round, from the top), then one sweep in column order that keeps what is above it and the first of those equal.
 template <typename T, int THREADS>
-__device__ __noinline__ void select_by_digits(const T *z, int first, int valid, int kept, unsigned long long *list,
+__device__ __noinline__ void select_by_digits(const T *z, int first, int valid, unsigned int kept, unsigned long long *list,
                                               unsigned int *bins)
 {
     __shared__ unsigned int warp_above[THREADS / 32], warp_equal[THREADS / 32];
@@ -165,7 +165,7 @@ __device__ __noinline__ void select_by_digits(const T *z, int first, int valid, 
         const unsigned int before = (1u << lane) - 1u;
         at_above += __popc(ba & before);
         at_equal += __popc(be & before);
-        if (is_above)
+        if (is_above && at_above < kept)        // they are fewer, unless a copy that was given up changes the row meanwhile
         {
             list[at_above] = entry_of(key, first + v);
         }
@@ -194,8 +194,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     __shared__ float warp_m[WARPS], warp_s[WARPS];
     __shared__ float2 block_ms[2];              // of two rows: this segment's maximum and sum
     __shared__ int collected, met;              // columns that reach, vectors that hold some
-    __shared__ unsigned int lost;               // a copy of this block's never came (1 + its phase): its rows from there on are not looked at
-    __shared__ int failed[2];                   // of two rows: some block of the cluster has not got its segment
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const cg::cluster_group cluster = cg::this_cluster();
     const int blocks = plan.cluster, rank = blocks > 1 ? static_cast<int>(cluster.block_rank()) : 0;
@@ -214,14 +212,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     unsigned long long *const best0 = list + a.room + a.room / 2;
     unsigned long long *const others = best0 + 2 * a.k;     // every segment's, brought over where they are few
     const bool brought = blocks * a.k <= MOST_BROUGHT;
+    unsigned int phase = 0u;                    // of row_bar, with what RowTile::wait adds
     auto start = [&](long long row) {
-        tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.vocab, &row_bar, lost == 0u,
-                   row == a.starved && rank == blocks - 1 ? 16u : 0u);
+        tile.start(static_cast<const T *>(a.logits) + row * a.ld, first, plan.segment, a.vocab, a.vocab, &row_bar, phase,
+                   row == a.starved && rank == blocks - 1);
     };
     if (tid == 0)
     {
-        lost = 0u;
-        failed[0] = failed[1] = 0;
         row_barrier_init(&row_bar);
     }
     __syncthreads();
@@ -230,7 +227,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
         cluster.sync();                         // every block of the cluster runs before one reads of another
     }
 
-    unsigned int phase = 0;
     int parity = 0;
     long long row = blockIdx.x / blocks;
     if (row < a.rows)
@@ -240,29 +236,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
     for (; row < a.rows; row += clusters, parity ^= 1)
     {
         unsigned long long *const best = best0 + parity * a.k;
+        const int valid = tile.valid;
+        const int kept = min(a.k, valid);       // of this segment
         if (tid == 0)
         {
             collected = 0;
             met = 0;
         }
-        if (lost == 0u && !row_wait(&row_bar, phase))
-        {
-            lost = 1u + phase;
-            g_row_timeout = 1;
-        }
-        phase ^= 1u;
-        tile.finish();
+        tile.wait(&row_bar, phase);
         __syncthreads();
-        if (lost != 0u)
-        {
-            tile.valid = tile.vecs = 0;
-            if (tid < blocks)
-            {
-                (blocks > 1 ? cluster.map_shared_rank(failed, tid) : failed)[parity] = 1;
-            }
-        }
-        const int valid = tile.valid;
-        const int kept = min(a.k, valid);       // of this segment
 
         // maxima of the groups
         Vec16<T> group;
@@ -558,8 +540,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
             }
             __syncthreads();
         }
-        const bool none = failed[parity] != 0;
-        for (int j = tid; j < kept && !none; j += THREADS)
+        for (int j = tid; j < kept; j += THREADS)
         {
             const unsigned long long entry = best[j];
             int place = j;
@@ -592,10 +573,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
         }
         if (rank == 0)
         {
-            for (int j = tid + (none ? 0 : a.vocab); j < a.k; j += THREADS)
+            for (int j = a.vocab + tid; j < a.k; j += THREADS)
             {
-                a.indices[row * a.k + j] = -1;  // fewer columns than asked for, or no row
-                static_cast<T *>(a.values)[row * a.k + j] = from_float<T>(none ? NAN : -INFINITY);
+                a.indices[row * a.k + j] = -1;  // fewer columns than asked for
+                static_cast<T *>(a.values)[row * a.k + j] = minus_infinity<T>();
             }
             if (sums && tid == 0)
             {
@@ -612,16 +593,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const
                 }
                 // a row of nothing but -inf has the log of 0; +inf has itself
                 a.lse[row] = isinf(all) ? all : static_cast<float>(all * inv_t + log(total));
-                if (none)
-                {
-                    a.lse[row] = NAN;
-                }
             }
         }
     }
-    if (tid == 0 && lost != 0u)
+    if (tid == 0)
     {
-        row_wait(&row_bar, lost - 1u);          // shared memory is not handed back with a copy on its way
+        row_leave(&row_bar, phase);
     }
     if (blocks > 1)
     {

@@ -512,8 +512,8 @@ B200AMP_API int b200amp_tune_get(const char *key, int *value);
 /* *out = what gave up a bounded wait on the current device since the last call, as a bit mask:
  * 1 a shared-memory staged pass 2 waiting for a bulk copy that never completed, 2 a ZeRO-1
  * kernel waiting for another rank, 4 a loss kernel waiting for the copy of a row; 0 = nothing. Reading
- * clears it. Synchronises the device. The row whose copy did not come and those that the same blocks take
- * after it have NaN loss and gradient; in b200amp_top_logits NaN values and log-sum-exp, and columns -1.
+ * clears it. Synchronises the device. A block that gave up a row's copy has NaN in its logits' place from there
+ * on: its rows have NaN loss and gradient, in b200amp_top_logits NaN values and log-sum-exp.
  * After a nonzero answer the optimizer state of the step that gave up is not to be trusted. */
 B200AMP_API int b200amp_device_error(int *out);
 /* Kernel launches enqueued by this library on the calling process so far. */

@@ -296,6 +296,16 @@ __device__ __forceinline__ void sweep_gradient(const RowTile<T, THREADS> &tile, 
     }
 }
 
+// Zeros from `from` to `to`, by a warp. A call, for rows that hardly occur.
+template <typename T>
+__device__ __noinline__ void zero_columns(T *out, int from, int to)
+{
+    for (int i = from + (threadIdx.x & 31); i < to; i += 32)
+    {
+        out[i] = from_float<T>(0.0f);
+    }
+}
+
 // A cluster a row, the row in its shared memory between the sweeps. A block has SWEEP threads that sweep the segment
 // and one more warp for what there is one of a row: the listed columns' sums, the factors, the loss. That warp works
 // while the others sweep, so its fp64 chains are off the row's path, and they are issued once a block and not once a
@@ -787,6 +797,11 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                     g = fmaf(shifted_fast(rec_z[j], m, c_1), l_1, g);
                 }
                 out[v] = from_float<T>(hard && v == y ? g - hard_scale : g);
+            }
+            if (a.cols > a.vocab && !(isfinite(shared_f_t + shared_f_1)))
+            {
+                // the padding, where 0 times the factor is NaN
+                zero_columns(out, max(first, a.vocab), min(first + plan.segment, a.cols));
             }
             if (lane == 0 && label_in && !listed_y && y >= first && y < first + valid)
             {

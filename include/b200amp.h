@@ -459,10 +459,10 @@ B200AMP_API int b200amp_top_logits(const void *logits, int dtype, long long rows
  *   - indices < 0 are empty slots. A row without any listed mass has KL 0. A column listed twice has the
  *     sum of its masses. If the student gives every column not listed no probability at all (or there
  *     is none), the rest term is left out.
- *   - An index or a label beyond the vocabulary is not read: the row's loss and gradient are NaN, so the
- *     step is skipped. NaN, +inf or nothing but -inf in a row of logits, or NaN in its record, do the
- *     same. A single -inf logit has probability 0 and gradient 0; where it has teacher mass or is the
- *     label, the loss is +inf and the gradient finite.
+ *   - An index or a label beyond the vocabulary is not read: the row's loss and its gradient (columns 0 ..
+ *     vocab - 1) are NaN, so the step is skipped. NaN, +inf or nothing but -inf in a row of logits, or
+ *     NaN in its record, do the same. A single -inf logit has probability 0 and gradient 0; where it has
+ *     teacher mass or is the label, the loss is +inf and the gradient finite.
  *   - k == 0 or soft_weight == 0: the cross-entropy alone (values, indices and lse may be null).
  *   - dlogits null: the loss alone. dlogits may be the logits themselves (same ld).
  * values[rows][k] has type value_dtype, indices[rows][k] int32, lse[rows] fp32. rows >= 0, 0 <= k <= 1024,

@@ -1,0 +1,44 @@
+"""What include/b200amp.h says of the losses where a row has no answer, and where a call has more than one user."""
+import math
+
+import pytest
+import torch
+
+import test_gpu_losses as L
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", list(L.TYPES))
+@pytest.mark.parametrize("hard,T", [(0.0, 1.0), (0.5, 1.0), (0.5, 2.0)])
+@pytest.mark.parametrize("vocab,cols,ld,dld", [(9, 13, 13, 13), (13, 16, 16, 16), (4098, 4160, 4160, 4160), (4097, 4103, 4103, 4104),
+                                               (50257, 50304, 50304, 50304), (131072, 131100, 131100, 131100)])
+def test_a_bad_row_is_nan_in_all_its_columns_and_0_in_its_padding(vocab, cols, ld, dld, hard, T, dtype):
+    rows = 12
+    p = L._problem(rows, vocab, cols, L.TYPES[dtype], 3, T, True, hard)
+    p["logits"][0, vocab - 1] = math.nan
+    p["logits"][1, int(p["indices"][1, 0])] = math.nan
+    p["logits"][2, 1] = math.inf
+    p["logits"][3, :] = -math.inf
+    p["indices"][4, 2] = vocab
+    p["indices"][5, 0] = 2 ** 31 - 1
+    p["values"][6, 1] = math.nan
+    p["targets"][7] = vocab if hard else int(p["targets"][7])   # without a hard weight the label is not looked at
+    p["logits"][8, vocab:] = math.nan                           # the padding is not read
+    p["logits"][9, vocab:] = math.inf
+    bad = torch.tensor([True] * 7 + [bool(hard)] + [False] * 4)
+    got = L._run(p, ld=ld, dld=dld)
+    assert torch.equal(torch.isnan(got["row_loss"]), bad)
+    nan = torch.isnan(got["dlogits"].float())
+    assert bool(nan[bad, :vocab].all()) and not bool(nan[~bad].any()) and not bool(got["dlogits"][:, vocab:].any())
+    assert math.isnan(got["loss"])
+    good = {**p, **{n: p[n][~bad] for n in ("logits", "targets", "values", "indices", "lse")}}
+    want = L._want(good)["row_loss"]
+    assert bool(((got["row_loss"][~bad].double() - want).abs() <= L._rel(vocab, 90.0) * (T * T + hard) + 2 * L.U * want.abs()).all())
+
+
+def test_a_loss_scale_beyond_fp32_leaves_the_padding_0():
+    p = L._problem(3, 500, 520, torch.float32, 4, 1.0, True, 2.0)
+    p["soft"] = 100.0
+    got = L._run(p, scale=2.0 ** 127)
+    assert not bool(got["dlogits"][:, 500:].any()) and not bool(torch.isfinite(got["dlogits"][:, :500]).all())

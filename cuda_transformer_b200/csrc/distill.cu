@@ -103,6 +103,13 @@ __device__ __forceinline__ float warp_max_once(float v)
     return m;
 }
 
+// a / b: to the nearest for fp32 gradients, to 2 ulp for 16-bit ones, whose own rounding is a thousand times that
+template <typename T>
+__device__ __forceinline__ float quotient(float a, float b)
+{
+    return sizeof(T) == 4 ? a / b : __fdividef(a, b);
+}
+
 // Sum over the first n lanes (a power of two), in every lane.
 template <typename V>
 __device__ __forceinline__ V sum_lanes(V v, int n)
@@ -327,9 +334,14 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
     namespace cg = cooperative_groups;
     using Tile = RowTile<T, SWEEP>;
     constexpr int THREADS = SWEEP + 32, WARPS = SWEEP / 32;     // WARPS: those that sweep
+    // fp32 gradients: the listed columns' and the label's, most of a gradient's magnitude, are worked out in fp64, as their
+    // terms cancel where student and teacher agree; a 16-bit one hides the difference (2^-12 against 2^-22).
+    constexpr bool WIDE = sizeof(T) == 4;
     extern __shared__ __align__(16) char dynamic[];
     __shared__ double scratch[THREADS / 32];
     __shared__ float shared_ref, shared_f_t, shared_f_1, t_max_of[WARPS];
+    __shared__ double shared_scale[2];          // loss scale over rows that count, times the weights (soft: over T too)
+    __shared__ double wide[4];                  // l_t and l_1 in fp64, what a mass is multiplied by, the label's gradient
     __shared__ int label_listed[2], beyond_listed[2];
     __shared__ uint64_t row_bar;
     __shared__ int last_block;
@@ -680,9 +692,9 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                 const float u_in_all_1 = two ? shifted_fast(all_u, m, c_1) : u_in_o * o_in_all;
                 not_y_1 = fmaf(u_1, u_in_all_1, listed_1);                      // all but the label, where that is not listed
                 total_1 = not_y_1 + (listed_y ? 0.0f : shifted_fast(z_y, m, c_1));
-                const float q_per = soft_scale * __fdividef(whole, total);
-                per_o = q_per * o_in_all - (rest > 0.0 ? soft_scale * __fdividef(static_cast<float>(rest), others) : 0.0f);
-                l_1 = hard ? __fdividef(hard_scale, total_1) : 0.0f;
+                const float q_per = soft_scale * quotient<T>(whole, total);
+                per_o = q_per * o_in_all - (rest > 0.0 ? soft_scale * quotient<T>(static_cast<float>(rest), others) : 0.0f);
+                l_1 = hard ? quotient<T>(hard_scale, total_1) : 0.0f;
                 l_t = q_per + (two ? 0.0f : l_1);
                 const float f_1 = l_1 * u_in_all_1;
                 if (lane == 0)
@@ -695,8 +707,9 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                 }
                 both_barrier<THREADS>();        // factors
 
-                // while the gradient is swept: the loss, in fp64, in turn by the cluster's blocks
-                if (rank == static_cast<int>(row / clusters & (blocks - 1)))
+                // while the gradient is swept: the row in fp64, for the loss (in turn by the cluster's blocks) and for WIDE
+                const bool turn = rank == static_cast<int>(row / clusters & (blocks - 1));
+                if (WIDE || turn)
                 {
                     double u_t64 = 0.0, u_164 = 0.0;
                     for (int i = lane; i < n_warps; i += 32)
@@ -721,14 +734,27 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
                     const double y_in_all64 = __shfl_sync(0xffffffffu, e, 20);
                     const double o = u_t64 * u_in_o64 + (listed_y ? 0.0 : y_in_o64);
                     const double s = o * o_in_all64 + listed_t64;
-                    const double s_1 = u_164 * (two ? u_in_all64 : u_in_o64 * o_in_all64) + listed_164 + (listed_y ? 0.0 : y_in_all64);
+                    const double not_y = u_164 * (two ? u_in_all64 : u_in_o64 * o_in_all64) + listed_164;
+                    const double s_1 = not_y + (listed_y ? 0.0 : y_in_all64);
+                    if (WIDE)
+                    {
+                        const double soft64 = shared_scale[0], hard64 = shared_scale[1], q = soft64 * (mass + rest) / s;
+                        const double by_label = hard64 / s_1;
+                        if (lane == 0)
+                        {
+                            wide[0] = q + (two ? 0.0 : by_label);
+                            wide[1] = by_label;
+                            wide[2] = a.lse != nullptr || own == 0.0 ? soft64 : soft64 / own;
+                            wide[3] = (q * o_in_all64 - (rest > 0.0 ? soft64 * rest / o : 0.0)) * y_in_o64 - by_label * not_y;
+                        }
+                    }
                     // one logarithm a lane
                     const double of = lane == 0 ? s : lane == 1 ? s_1 : lane == 2 ? o : lane == 3 ? rest : own;
                     const double log_of = of > 0.0 ? log(of) : 0.0;
                     const double log_s = __shfl_sync(0xffffffffu, log_of, 0), log_s1 = __shfl_sync(0xffffffffu, log_of, 1);
                     const double log_o = __shfl_sync(0xffffffffu, log_of, 2), log_rest = __shfl_sync(0xffffffffu, log_of, 3);
                     const double log_own = __shfl_sync(0xffffffffu, log_of, 4);
-                    if (lane == 0)
+                    if (lane == 0 && turn)
                     {
                         double loss = 0.0;
                         if (a.k > 0)
@@ -783,6 +809,11 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
             const double scale = static_cast<double>(a.st->loss_scale) / static_cast<double>(n_valid > 0 ? n_valid : 1);
             soft_scale = a.k > 0 ? static_cast<float>(scale * a.soft * inv_t) : 0.0f;
             hard_scale = hard ? static_cast<float>(scale * a.hard) : 0.0f;
+            if (WIDE && tid == SWEEP)           // of the warp that reads it
+            {
+                shared_scale[0] = a.k > 0 ? scale * a.soft * inv_t : 0.0;
+                shared_scale[1] = hard ? scale * a.hard : 0.0;
+            }
         }
         if (!sweeps && y >= 0 && out != nullptr)
         {
@@ -791,6 +822,13 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
             for (int i = lane; i < n_listed; i += 32)
             {
                 const int j = mine[i], v = rec_col[j];
+                if (WIDE)
+                {
+                    double g64 = shifted(rec_z[j], m, inv_t) * wide[0] - wide[2] * rec_w[j];
+                    g64 += two ? shifted(rec_z[j], m, 1.0) * wide[1] : 0.0;
+                    out[v] = from_float<T>(static_cast<float>(hard && v == y ? g64 - shared_scale[1] : g64) + poison);
+                    continue;
+                }
                 float g = fmaf(shifted_fast(rec_z[j], m, c_t), l_t, -p_scale * static_cast<float>(rec_w[j])) + poison;
                 if (two)
                 {
@@ -805,7 +843,8 @@ __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(c
             }
             if (lane == 0 && label_in && !listed_y && y >= first && y < first + valid)
             {
-                out[y] = from_float<T>(per_o * y_in_o - hard_scale * __fdividef(not_y_1, total_1) + poison);
+                out[y] = from_float<T>((WIDE ? static_cast<float>(wide[3])
+                                             : per_o * y_in_o - hard_scale * __fdividef(not_y_1, total_1)) + poison);
             }
         }
         y = next_y;

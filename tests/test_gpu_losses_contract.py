@@ -42,3 +42,23 @@ def test_a_loss_scale_beyond_fp32_leaves_the_padding_0():
     p["soft"] = 100.0
     got = L._run(p, scale=2.0 ** 127)
     assert not bool(got["dlogits"][:, 500:].any()) and not bool(torch.isfinite(got["dlogits"][:, :500]).all())
+
+
+@pytest.mark.parametrize("vocab", [2, 7, 100, 999])
+@pytest.mark.parametrize("T,hard", [(1.0, 0.0), (1.0, 0.5), (2.0, 0.5), (0.7, 0.0)])
+@pytest.mark.parametrize("rest", [False, True])
+def test_fp32_gradients_of_listed_columns_are_rounded_once(rest, T, hard, vocab):
+    """Student and teacher agree but for a hundredth, so each gradient is a small difference of two terms. All columns are
+    listed, or all but the label's: no fp32 sum enters. Each term is off by at most 2^-40 of itself (sums of up to 999 terms
+    in 64 bits: 2^-43; powers of up to 20: 2^-47), the gradient then by half a step of fp32."""
+    p = L._problem(9, vocab, vocab, torch.float32, vocab, T, rest, hard, seed=vocab)
+    gen = torch.Generator().manual_seed(vocab)
+    teacher = torch.zeros(9, vocab).scatter_(1, p["indices"].long(), p["values"])
+    p["logits"] = teacher + 0.01 * torch.randn(9, vocab, generator=gen)
+    if hard and rest:
+        for i in range(9):                                      # the label's column is not listed
+            p["indices"][i][p["indices"][i] == p["targets"][i]] = -1
+    got, want = L._run(p), L._want(p)
+    limit = want["dlogits"].abs() * L.U + want["size"] * 2.0 ** -40 + L.TINY[torch.float32]
+    err = (got["dlogits"].double() - want["dlogits"]).abs()
+    assert bool((err <= limit).all()), float((err / limit).max())

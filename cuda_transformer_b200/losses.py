@@ -158,14 +158,17 @@ def balance_loss(logits: torch.Tensor, dlogits: Optional[torch.Tensor], chosen: 
 
 class LossCalls:
     """The losses on an optimizer's own step state: mixed into the owners of amp.py, which provide state and
-    loss_workspace (both on the optimizer's device)."""
+    loss_workspace (both on the optimizer's device). That workspace serves one stream at a time, like any other: calls
+    whose GPU work may overlap (streams side by side, two graphs replayed at once) each bring a `workspace` of their
+    own (loss_workspace()). Calls that write or add to state.loss are to follow one another in any case."""
 
     def distill_loss(self, logits, dlogits, targets, values, indices, lse, row_loss, vocab=None, temperature=1.0,
-                     soft_weight=1.0, hard_weight=0.0, stream=None) -> None:
-        distill_loss(logits, dlogits, targets, values, indices, lse, self.state, row_loss, self.loss_workspace, vocab,
-                     temperature, soft_weight, hard_weight, stream)
+                     soft_weight=1.0, hard_weight=0.0, stream=None, workspace=None) -> None:
+        distill_loss(logits, dlogits, targets, values, indices, lse, self.state, row_loss,
+                     self.loss_workspace if workspace is None else workspace, vocab, temperature, soft_weight, hard_weight,
+                     stream)
 
     def balance_loss(self, logits, dlogits, chosen, targets, counts, loss, weight=0.01, accumulate=False,
-                     add_to_state=True, stream=None) -> None:
-        balance_loss(logits, dlogits, chosen, targets, self.state, counts, loss, self.loss_workspace, weight,
-                     accumulate, add_to_state, stream)
+                     add_to_state=True, stream=None, workspace=None) -> None:
+        balance_loss(logits, dlogits, chosen, targets, self.state, counts, loss,
+                     self.loss_workspace if workspace is None else workspace, weight, accumulate, add_to_state, stream)

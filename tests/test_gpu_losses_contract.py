@@ -62,3 +62,26 @@ def test_fp32_gradients_of_listed_columns_are_rounded_once(rest, T, hard, vocab)
     limit = want["dlogits"].abs() * L.U + want["size"] * 2.0 ** -40 + L.TINY[torch.float32]
     err = (got["dlogits"].double() - want["dlogits"]).abs()
     assert bool((err <= limit).all()), float((err / limit).max())
+
+
+def test_an_optimizers_calls_on_two_streams_with_a_workspace_each():
+    """Two layers' routers at once, each on its stream, on one optimizer's state (read only: nothing is added to its loss)."""
+    from cuda_transformer_b200 import losses
+    opt, _, _ = L._step_case()
+    layers = []
+    for seed in (1, 2):
+        z, chosen, targets = L._balance_problem(20011, 60, torch.float32, 4, 0.2, 0.1, seed=seed)
+        layers.append(dict(z=z.cuda(), c=chosen.cuda(), y=targets.cuda(), d=torch.empty(20011, 60, device="cuda"),
+                           counts=torch.empty(60, dtype=torch.int32, device="cuda"), loss=torch.empty(1, device="cuda"),
+                           ws=losses.loss_workspace(), s=torch.cuda.Stream()))
+    alone = []
+    for q in layers:
+        opt.balance_loss(q["z"], q["d"], q["c"], q["y"], q["counts"], q["loss"], add_to_state=False)
+        alone.append([q[n].clone() for n in ("d", "counts", "loss")])
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for q in layers:
+            opt.balance_loss(q["z"], q["d"], q["c"], q["y"], q["counts"], q["loss"], add_to_state=False, stream=q["s"], workspace=q["ws"])
+    torch.cuda.synchronize()
+    for q, want in zip(layers, alone):
+        assert all(torch.equal(q[n], w) for n, w in zip(("d", "counts", "loss"), want)) and not bool(q["ws"][:L.COUNTERS].any())

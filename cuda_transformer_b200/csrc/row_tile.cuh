@@ -33,11 +33,6 @@ struct RowPlan
 template <typename More>
 int plan_rows(long long rows, int cols, int size, int least, int most, More more, RowPlan *plan)
 {
-    const int sms = sm_count();
-    if (sms <= 0)
-    {
-        return B200AMP_ERR_CUDA;
-    }
     auto fill = [&](int cluster, int threads) {
         plan->cluster = cluster;
         plan->threads = threads;
@@ -59,6 +54,17 @@ int plan_rows(long long rows, int cols, int size, int least, int most, More more
     {
         cluster *= 2;
     }
+    if (plan->smem > MAX_ROW_SMEM)
+    {
+        set_error("rows of %d columns with what they list need %d bytes of shared memory in each of %d blocks, at most %d", cols,
+                  plan->smem, MAX_CLUSTER, MAX_ROW_SMEM);
+        return B200AMP_ERR_LIMIT;
+    }
+    const int sms = sm_count();
+    if (sms <= 0)
+    {
+        return B200AMP_ERR_CUDA;
+    }
     // A handful of rows: long ones are worth spreading over SMs that would stand idle.
     while (cluster < 4 && rows * cluster < sms && plan->segment > 16384)
     {
@@ -78,11 +84,6 @@ int plan_rows(long long rows, int cols, int size, int least, int most, More more
     if (plan->smem > 112 * 1024)
     {
         fill(cluster, most);
-    }
-    if (plan->smem > MAX_ROW_SMEM)
-    {
-        set_error("rows of %d columns need %d bytes of shared memory a block", cols, plan->smem);
-        return B200AMP_ERR_LIMIT;
     }
     return B200AMP_OK;
 }

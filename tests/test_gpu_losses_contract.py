@@ -85,3 +85,15 @@ def test_an_optimizers_calls_on_two_streams_with_a_workspace_each():
     torch.cuda.synchronize()
     for q, want in zip(layers, alone):
         assert all(torch.equal(q[n], w) for n, w in zip(("d", "counts", "loss"), want)) and not bool(q["ws"][:L.COUNTERS].any())
+
+
+@pytest.mark.parametrize("dtype,vocab,k", [("f16", 1_200_000, 1024), ("f32", 600_000, 1024), ("bf16", 1_660_000, 3), ("f32", 850_000, 3)])
+def test_the_longest_rows(dtype, vocab, k):
+    p = L._problem(2, vocab, vocab, L.TYPES[dtype], k, 1.0, True, 0.5)
+    L._check(p, L._run(p))
+    z = p["logits"]
+    values, indices, lse = L._top(z, k)
+    want = torch.sort(z.float(), dim=1, descending=True, stable=True)
+    assert torch.equal(indices.long(), want.indices[:, :k]) and torch.equal(values.float(), want.values[:, :k])
+    exact = torch.logsumexp(z.double(), dim=1)
+    assert bool(((lse.double() - exact).abs() <= L._rel(vocab, 30.0) + 2 * L.U * exact.abs()).all())

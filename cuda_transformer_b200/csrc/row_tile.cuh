@@ -308,10 +308,6 @@ struct RowTile
     {
         return reinterpret_cast<T *>(buf) + lead + (column - first);
     }
-    __device__ __forceinline__ bool holds(int column) const
-    {
-        return column >= first && column < first + valid;
-    }
     __device__ __forceinline__ Vec16<T> vec(int i) const
     {
         return reinterpret_cast<const Vec16<T> *>(buf)[i];

@@ -326,8 +326,8 @@ __device__ __noinline__ void zero_columns(T *out, int from, int to)
 // 8192 rows of 50257 fp16 columns (k 64, rest and label) take 350 us, 1.6 GB, 4.6 TB/s; the powers alone would take 181 us
 // of the special function unit, the bytes 246 us. A block's rows are behind one another, so what bounds it is a row's
 // chain: at two blocks an SM about 20,000 cycles, 6,500 for the sums, 5,500 for the gradient, the rest barriers, the
-// record and the factors. Registers for two blocks of 256 threads an SM (or eight of 64): with fewer, spills go past
-// the little L1 that the rows leave (422 us).
+// record and the factors. Registers for two blocks of 256 threads an SM (96 a thread, no spills): with fewer, spills go past
+// the little L1 that the rows leave (422 us). Eight blocks of 64 have 80 a thread and spill 28 to 36 bytes.
 template <typename T, int SWEEP>
 __global__ void __launch_bounds__(SWEEP + 32, 512 / SWEEP) distill_rows_kernel(const DistillArgs a, const RowPlan plan)
 {

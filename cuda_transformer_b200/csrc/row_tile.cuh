@@ -46,9 +46,10 @@ int plan_rows(long long rows, int cols, int size, int least, int most, More more
         return B200AMP_ERR_LIMIT;
     }
     // The fewest blocks that hold the row: what there is one of a segment (its barriers, its listed columns, its exchange
-    // with the others) costs about as much as sweeping 10,000 columns, so fewer and longer segments win even where
-    // one block fills an SM (510 rows of 128,001 bf16 columns, top_logits: 2 blocks a row 160 us, 4 blocks 186 us; 8192
-    // rows of 50,304 fp16 columns, distill_loss: 1 block 351 us, 2 blocks 452 us).
+    // with the others) costs about as much as sweeping 10,000 columns, so fewer and longer segments win for 16-bit rows, even
+    // where one block fills an SM (510 rows of 128,001 bf16 columns, top_logits: 2 blocks a row 160 us, 4 blocks 186 us; 8192
+    // rows of 50,304 fp16 columns, distill_loss: 1 block 351 us, 2 blocks 452 us). For long fp32 rows it is about even (2048
+    // rows of 131,072, distill_loss: 4 blocks 593 us, 8 blocks 582 us).
     int cluster = 1;
     for (fill(1, 256); cluster < MAX_CLUSTER && plan->smem > MAX_ROW_SMEM; fill(cluster, 256))
     {
@@ -75,7 +76,7 @@ int plan_rows(long long rows, int cols, int size, int least, int most, More more
     // more and smaller blocks side by side (distill_loss, 8192 rows: of 700 fp16 columns 64 threads 59 us, 128 threads
     // 86 us, 256 threads 158 us; of 12,000 bf16 columns 117, 126 and 170 us), unless there are hardly rows for them; and
     // a block that has an SM to itself wants its threads (top_logits, 510 rows of 128,001 bf16 columns: 256 threads
-    // 160 us, 512 threads 121 us).
+    // 160 us, 512 threads 121 us), but not two that share one (8192 rows of 50,257 fp16 columns: 300 and 303 us).
     if (rows * cluster > 2ll * sms)
     {
         const int bytes = plan->segment * size;

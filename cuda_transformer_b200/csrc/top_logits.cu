@@ -177,9 +177,10 @@ __device__ __noinline__ void select_by_digits(const T *z, int first, int valid, 
     }
 }
 
-// A cluster a row. 8192 rows of 50257 fp16 columns, k 64: 317 us, 0.83 GB, 2.6 TB/s (the bytes alone 126 us, the powers
+// A cluster a row. 8192 rows of 50257 fp16 columns, k 64: 320 us, 0.83 GB, 2.6 TB/s (the bytes alone 126 us, the powers
 // 92 us). A row of a block takes about 20,000 cycles: 8,000 the second sweep, 3,000 the threshold, 2,000 each the
-// collection and the sorting, 1,500 the first sweep; the next row's copy is under the sorting.
+// collection and the sorting, 1,500 the first sweep; the next row's copy is under the sorting. 64 registers a thread, for two
+// blocks of 512 an SM or eight of 128, with 4 to 24 bytes of spills.
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) top_rows_kernel(const TopArgs a, const RowPlan plan)
 {
